@@ -127,6 +127,71 @@ RK_API rk_status rk_conv1d_fprop_static(const float* x, const float* w, const fl
  * each rk_conv1d_fprop_static call clears the word when it starts. */
 RK_API rk_status rk_conv1d_static_check(void* stream);
 
+/* ---- quantised linear layers and the norm that feeds them ------------------
+ * Stateless, like the conv seam: device pointers of the current device, work
+ * enqueued on `stream`, no synchronisation, no allocation (so calls may be
+ * captured into CUDA graphs), results that do not change from run to run.  No
+ * counterpart in the reference, whose linear layers are FP32 and TF32.
+ * Activations, norm weights and residuals are RK_DTYPE_* elements; every sum,
+ * norm and scale is held in 32 bits and rounded once, to nearest, when a result
+ * is stored.  Row pitches (ld*) count elements and are at least the row's
+ * length; a single row's pitch is not looked at.  rows = 0 does nothing.  An
+ * unsupported argument gives RK_ERR_CANNOT_IMPLEMENT and enqueues nothing.
+ *
+ * 8-bit rows ("q8"): e4m3 codes with one float scale a row, value = scale x
+ * code.  scale = max(max|y|, 1e-30) / 448, so a row of zeros has zero codes.  A
+ * NaN anywhere in a row gives a NaN scale. */
+#define RK_DTYPE_F32 0
+#define RK_DTYPE_F16 1
+#define RK_DTYPE_BF16 2
+
+/* Root-mean-square norm of h = x + residual (residual may be NULL: h = x):
+ * y = h / sqrt(mean(h^2) + eps) * weight over rows of `cols` elements, from the
+ * unrounded h.  sum_out (may be NULL) receives h in the input's type; it and y
+ * may be x or residual themselves (same pitch).  weight has cols elements of
+ * the same type.  _q8 writes 8-bit rows q [rows][cols] (pitch ldq bytes, a
+ * multiple of 16 where rk_linear_q8 reads them; bytes between cols and ldq are
+ * left as they are) and scale [rows]. */
+RK_API rk_status rk_rms_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight,
+                             void* sum_out, long long lds, void* y, long long ldy, int rows, int cols, float eps,
+                             int dtype, void* stream);
+RK_API rk_status rk_rms_norm_q8(const void* x, long long ldx, const void* residual, long long ldr,
+                                const void* weight, void* sum_out, long long lds, void* q, long long ldq,
+                                float* scale, int rows, int cols, float eps, int dtype, void* stream);
+/* 8-bit rows of x itself: weights when they are loaded, activations that no norm precedes. */
+RK_API rk_status rk_quantize_q8(const void* x, long long ldx, void* q, long long ldq, float* scale, int rows,
+                                int cols, int dtype, void* stream);
+
+/* Linear layer on 8-bit rows (tcgen05 e4m3 products, FP32 accumulation):
+ * y[rows][n] = x w^T + bias + residual with x [rows][k] and w [n][k] 8-bit rows
+ * as above (16-byte aligned, pitches multiples of 16), bias [n] float or NULL,
+ * residual [rows][n] in y's type or NULL (may be y itself). */
+RK_API rk_status rk_linear_q8(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
+                              const float* w_scale, const float* bias, const void* residual, long long ldr, void* y,
+                              long long ldy, int rows, int n, int k, int dtype, void* stream);
+
+/* 4-bit weights ("q4"): code q in 0..15 stands for scale x (q - zero), scale
+ * and zero per row and group of `group` columns (32, 64 or a multiple of 128;
+ * the last group may be short).  Byte j of a row holds column 2j in its low and
+ * 2j + 1 in its high half; a row takes ceil(k / 32) x 16 bytes (what lies past
+ * column k is ignored) and starts on a 16-byte boundary.  scales
+ * [n][ceil(k / group)] of type scale_dtype; zeros, the same shape in bytes
+ * (0..15), or NULL: 8.
+ * rk_quantize_q4 makes them from w [n][k] of type dtype: with zeros the codes
+ * span [min(w, 0), max(w, 0)] of the group, else scale = max|w| / 7; w must be
+ * finite.
+ * rk_linear_q4: y[rows][n] = x w^T + bias + residual, x and y of type dtype
+ * (32-bit x keeps its precision: x is split into exact 16-bit parts), bias
+ * float or NULL, residual in y's type or NULL (may be y itself).  Meant for few
+ * rows, where the weights' bytes are the cost; any number of rows is right, and
+ * beyond a few dozen rk_linear_q8 or the conv seam are faster. */
+RK_API rk_status rk_quantize_q4(const void* w, long long ldw, void* q, long long ldq, void* scales, uint8_t* zeros,
+                                int n, int k, int group, int dtype, int scale_dtype, void* stream);
+RK_API rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
+                              const uint8_t* zeros, const float* bias, const void* residual, long long ldr, void* y,
+                              long long ldy, int rows, int n, int k, int group, int dtype, int scale_dtype,
+                              void* stream);
+
 /* ---- model context ------------------------------------------------------- */
 RK_API rk_status rk_create(int device, const rk_options* opts, rk_ctx** out);
 RK_API void rk_destroy(rk_ctx* ctx);

@@ -15,12 +15,18 @@ LIB_PATH = os.path.join(HERE, "librokoko_b200.so")
 RK_OK = 0
 RK_PRECISION_FP32 = 0
 RK_PRECISION_FP16 = 1
+RK_DTYPE_F32 = 0
+RK_DTYPE_F16 = 1
+RK_DTYPE_BF16 = 2
+RK_ERR_CANNOT_IMPLEMENT = -1
 RK_ERR_WORKSPACE = -2
 RK_ERR_DEVICE_TIMEOUT = -7
 RK_CONV_STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 
 _f32p = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
+_p = ctypes.c_void_p
+_ll = ctypes.c_longlong
 _lib = None
 
 
@@ -53,6 +59,16 @@ SIGNATURES = [
     ("rk_conv1d_fprop_f16", ctypes.c_int,
      [ctypes.c_void_p] * 5 + [ctypes.c_void_p, ctypes.c_size_t] + [ctypes.c_int] * 7 + [ctypes.c_void_p]),
     ("rk_conv1d_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 7),
+    ("rk_rms_norm", ctypes.c_int,
+     [_p, _ll, _p, _ll, _p, _p, _ll, _p, _ll, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int, _p]),
+    ("rk_rms_norm_q8", ctypes.c_int,
+     [_p, _ll, _p, _ll, _p, _p, _ll, _p, _ll, _p, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int, _p]),
+    ("rk_quantize_q8", ctypes.c_int, [_p, _ll, _p, _ll, _p, ctypes.c_int, ctypes.c_int, ctypes.c_int, _p]),
+    ("rk_linear_q8", ctypes.c_int,
+     [_p, _ll, _p, _p, _ll, _p, _p, _p, _ll, _p, _ll] + [ctypes.c_int] * 4 + [_p]),
+    ("rk_quantize_q4", ctypes.c_int, [_p, _ll, _p, _ll, _p, _p] + [ctypes.c_int] * 5 + [_p]),
+    ("rk_linear_q4", ctypes.c_int,
+     [_p, _ll, _p, _ll, _p, _p, _p, _p, _ll, _p, _ll] + [ctypes.c_int] * 6 + [_p]),
     ("rk_create", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(rk_options), ctypes.POINTER(ctypes.c_void_p)]),
     ("rk_destroy", None, [ctypes.c_void_p]),
     ("rk_load_weights_koko", ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]),

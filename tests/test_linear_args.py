@@ -1,0 +1,117 @@
+"""Argument checks of the quantised linear layers and norms at the C ABI (no
+GPU): every unsupported argument is refused with a status and a reason before
+any CUDA call, and zero rows are no work.  The pointers are never read."""
+import ctypes
+
+import pytest
+
+P = 1 << 20  # a 16-byte aligned address that nothing dereferences
+F32, F16, BF16 = 0, 1, 2
+REFUSED = -1
+
+
+def _norm(L, name="rk_rms_norm", x=P, ldx=64, res=None, ldr=0, w=P, h=None, ldh=0, y=P, ldy=64, rows=4, cols=64,
+          dtype=F32, scale=P):
+    if name == "rk_rms_norm":
+        return L.rk_rms_norm(x, ldx, res, ldr, w, h, ldh, y, ldy, rows, cols, 1e-6, dtype, None)
+    if name == "rk_rms_norm_q8":
+        return L.rk_rms_norm_q8(x, ldx, res, ldr, w, h, ldh, y, ldy, scale, rows, cols, 1e-6, dtype, None)
+    return L.rk_quantize_q8(x, ldx, y, ldy, scale, rows, cols, dtype, None)
+
+
+NORM_BAD = [dict(x=None), dict(y=None), dict(cols=0), dict(rows=-1), dict(dtype=3), dict(dtype=-1), dict(ldx=63),
+            dict(ldy=63), dict(x=P + 2), dict(x=P + 1, dtype=BF16)]
+
+
+@pytest.mark.parametrize("name", ["rk_rms_norm", "rk_rms_norm_q8", "rk_quantize_q8"])
+@pytest.mark.parametrize("bad", NORM_BAD, ids=str)
+def test_norm_refuses(rk_lib, name, bad):
+    assert _norm(rk_lib, name, **bad) == REFUSED
+    assert name.encode() in rk_lib.rk_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(w=None), dict(res=P, ldr=10), dict(h=P, ldh=10), dict(w=P + 2), dict(h=P + 3, ldh=64)],
+                         ids=str)
+def test_norm_refuses_residual_and_weight(rk_lib, bad):
+    assert _norm(rk_lib, "rk_rms_norm", **bad) == REFUSED
+    assert _norm(rk_lib, "rk_rms_norm_q8", **bad) == REFUSED
+
+
+def test_q8_rows_need_a_scale(rk_lib):
+    assert _norm(rk_lib, "rk_rms_norm_q8", scale=None) == REFUSED
+    assert _norm(rk_lib, "rk_quantize_q8", scale=None) == REFUSED
+    assert _norm(rk_lib, "rk_quantize_q8", scale=P + 1) == REFUSED
+
+
+def _q8(L, x=P, ldx=64, sx=P, w=P, ldw=64, sw=P, b=None, r=None, ldr=0, y=P, ldy=32, rows=4, n=32, k=64, dtype=F32):
+    return L.rk_linear_q8(x, ldx, sx, w, ldw, sw, b, r, ldr, y, ldy, rows, n, k, dtype, None)
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(sx=None), dict(w=None), dict(sw=None), dict(y=None), dict(ldx=48),
+                                 dict(ldw=48), dict(ldy=31), dict(r=P, ldr=31), dict(rows=-1), dict(n=0), dict(k=0),
+                                 dict(dtype=3), dict(x=P + 8), dict(w=P + 8), dict(ldx=72), dict(ldw=72), dict(y=P + 2),
+                                 dict(b=P + 2), dict(r=P + 2, ldr=32)], ids=str)
+def test_linear_q8_refuses(rk_lib, bad):
+    assert _q8(rk_lib, **bad) == REFUSED
+    assert b"rk_linear_q8" in rk_lib.rk_last_error()
+
+
+def _q4(L, x=P, ldx=96, w=P, ldw=48, s=P, z=None, b=None, r=None, ldr=0, y=P, ldy=32, rows=4, n=32, k=96, group=32,
+        dtype=F32, sdtype=F32):
+    return L.rk_linear_q4(x, ldx, w, ldw, s, z, b, r, ldr, y, ldy, rows, n, k, group, dtype, sdtype, None)
+
+
+Q4_BAD = [dict(x=None), dict(w=None), dict(s=None), dict(y=None), dict(ldx=95), dict(ldw=32), dict(ldw=56), dict(ldy=31),
+          dict(rows=-1), dict(n=0), dict(k=0), dict(dtype=3), dict(sdtype=3), dict(group=0), dict(group=16),
+          dict(group=96), dict(group=192), dict(group=-128), dict(w=P + 8), dict(x=P + 2), dict(s=P + 2),
+          dict(r=P, ldr=31), dict(b=P + 1)]
+
+
+@pytest.mark.parametrize("bad", Q4_BAD, ids=str)
+def test_linear_q4_refuses(rk_lib, bad):
+    assert _q4(rk_lib, **bad) == REFUSED
+    assert b"rk_linear_q4" in rk_lib.rk_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(w=None), dict(q=None), dict(s=None), dict(ldw=95), dict(ldq=32), dict(ldq=56),
+                                 dict(n=-1), dict(k=0), dict(group=48), dict(dtype=4), dict(sdtype=4), dict(q=P + 4),
+                                 dict(n=1 << 30, k=1 << 20, ldw=1 << 20, ldq=1 << 19)], ids=str)
+def test_quantize_q4_refuses(rk_lib, bad):
+    a = dict(w=P, ldw=96, q=P, ldq=48, s=P, z=None, n=32, k=96, group=32, dtype=F32, sdtype=F32) | bad
+    assert rk_lib.rk_quantize_q4(a["w"], a["ldw"], a["q"], a["ldq"], a["s"], a["z"], a["n"], a["k"], a["group"],
+                                 a["dtype"], a["sdtype"], None) == REFUSED
+    assert b"rk_quantize_q4" in rk_lib.rk_last_error()
+
+
+def test_zero_rows_are_no_work(rk_lib):
+    for name in ("rk_rms_norm", "rk_rms_norm_q8", "rk_quantize_q8"):
+        assert _norm(rk_lib, name, rows=0, x=None, y=None) == 0
+    assert _q8(rk_lib, rows=0, x=None, y=None) == 0
+    assert _q4(rk_lib, rows=0, x=None, y=None) == 0
+    assert rk_lib.rk_quantize_q4(None, 0, None, 0, None, None, 0, 96, 32, F32, F32, None) == 0
+
+
+def test_python_front_end_refuses_host_tensors():
+    torch = pytest.importorskip("torch")
+    from rokoko_b200 import linear
+    x, w = torch.zeros(4, 64), torch.ones(64)
+    with pytest.raises(ValueError, match="x: a CUDA tensor"):
+        linear.rms_norm(x, w)
+    with pytest.raises(ValueError, match="x: a CUDA tensor"):
+        linear.rms_norm_q8(x, w)
+    with pytest.raises(ValueError, match="x: a CUDA tensor"):
+        linear.quantize_q8(x)
+    with pytest.raises(ValueError, match="x: a CUDA tensor"):
+        linear.linear_q8(x, w, x, w)
+    with pytest.raises(ValueError, match="w: a CUDA tensor"):
+        linear.quantize_q4(x)
+    with pytest.raises(ValueError, match="x: a CUDA tensor"):
+        linear.linear_q4(x, x, x, 32)
+    with pytest.raises(ValueError, match="x: float32, float16 or bfloat16"):
+        linear.rms_norm(x.double(), w)
+
+
+def test_header_constants_match():
+    from rokoko_b200 import lib
+    assert (lib.RK_DTYPE_F32, lib.RK_DTYPE_F16, lib.RK_DTYPE_BF16) == (F32, F16, BF16)
+    assert ctypes.sizeof(ctypes.c_longlong) == 8
