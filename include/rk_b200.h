@@ -192,6 +192,12 @@ RK_API rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long 
                               long long ldy, int rows, int n, int k, int group, int dtype, int scale_dtype,
                               void* stream);
 
+/* Synchronises `stream` and reports (and clears) the error words of the
+ * operators above on the current device: RK_ERR_DEVICE_TIMEOUT when a bounded
+ * device-side wait of a call since the last check gave up (its output is then
+ * incomplete), else RK_OK.  The words are shared by all calls on a device. */
+RK_API rk_status rk_linear_check(void* stream);
+
 /* ---- model context ------------------------------------------------------- */
 RK_API rk_status rk_create(int device, const rk_options* opts, rk_ctx** out);
 RK_API void rk_destroy(rk_ctx* ctx);

@@ -55,7 +55,15 @@ void launch(const Q8Args& a, cudaStream_t st) {
     linear_q8_kernel<T><<<dim3((a.n + 15) / 16, gy < 65535 ? gy : 65535), 256, 0, st>>>(a);
 }
 
+__device__ uint32_t q8_err;  // set when a bounded wait of a kernel gives up
+
 }  // namespace
+
+void* q8_err_word() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, q8_err) == cudaSuccess ? p : nullptr;
+}
+
 }  // namespace rk
 
 using namespace rk;

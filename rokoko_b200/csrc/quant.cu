@@ -1,0 +1,46 @@
+// quant.cu -- what the quantised-serving operators share on the host: the SM
+// count, and rk_linear_check, which reads the device error words of their
+// bounded waits.
+#include "quant.cuh"
+
+#include <cstdio>
+
+#include "status.h"
+
+namespace rk {
+
+int sm_count() {
+    static int cache[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!cache[dev]) {
+        int n = 0;
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        cache[dev] = n > 0 ? n : 148;
+    }
+    return cache[dev];
+}
+
+}  // namespace rk
+
+extern "C" rk_status rk_linear_check(void* stream) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    void* words[] = {rk::norm_err_word(), rk::q8_err_word()};
+    uint32_t seen = 0;
+    for (void* p : words) {
+        uint32_t e = 0;
+        if (!p) return rk::fail_cuda(RK_ERR_CUDA, "rk_linear_check: cudaGetSymbolAddress");
+        if (cudaMemcpyAsync(&e, p, 4, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+            cudaStreamSynchronize(st) != cudaSuccess)
+            return rk::fail_cuda(RK_ERR_CUDA, "rk_linear_check");
+        if (e && (cudaMemsetAsync(p, 0, 4, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess))
+            return rk::fail_cuda(RK_ERR_CUDA, "rk_linear_check: clearing the error word");
+        if (e) seen = e;
+    }
+    if (seen) {
+        char buf[96];
+        snprintf(buf, sizeof buf, "device wait timed out (code %u)", seen);
+        return rk::fail(RK_ERR_DEVICE_TIMEOUT, buf);
+    }
+    return RK_OK;
+}

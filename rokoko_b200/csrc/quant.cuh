@@ -40,6 +40,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// SM count of the current device (148 when it cannot be asked)
+int sm_count();
+
+// Device addresses of the error words of the operators' bounded waits, on the current device.
+void* norm_err_word();
+void* q8_err_word();
+
 inline size_t dtype_bytes(int dtype) { return dtype == RK_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == RK_DTYPE_F32 || dtype == RK_DTYPE_F16 || dtype == RK_DTYPE_BF16; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

@@ -7,6 +7,9 @@
 //   q = e4m3(y / s),  s = max(max|y|, 1e-30) / 448
 #include <cuda_fp8.h>
 
+#include <atomic>
+
+#include "ptx.cuh"
 #include "quant.cuh"
 #include "status.h"
 
@@ -21,46 +24,360 @@ struct NormArgs {
     long long ldx, ldr, lds, ldy, ldq;
     int rows, cols;
     float eps;
+    float inv_cols;
+    uint32_t xoff, roff;  // x and res modulo 16 bytes
 };
 
-// Simple form: one block per row, the row read twice.
-template <typename T, bool NORM>
-__global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
-    __shared__ float red_s[8], red_m[8];
+__device__ uint32_t norm_err;  // set when a bounded wait of the streaming kernel gives up
+
+constexpr int RING_BYTES = 208 * 1024;  // shared memory of an SM that the streaming kernel's rings share
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+template <int VEC>
+struct alignas(VEC) Codes {
+    uint8_t v[VEC];
+};
+
+template <int VEC>
+__device__ __forceinline__ void store_codes(uint8_t* q, const float (&v)[VEC], float inv_scale) {
+    Codes<VEC> c;
+    if constexpr (VEC == 1) {
+        c.v[0] = __nv_cvt_float_to_fp8(v[0] * inv_scale, __NV_SATFINITE, __NV_E4M3);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const __nv_fp8x2_storage_t p =
+                __nv_cvt_float2_to_fp8x2(make_float2(v[j] * inv_scale, v[j + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3);
+            c.v[j] = (uint8_t)(p & 0xff);
+            c.v[j + 1] = (uint8_t)(p >> 8);
+        }
+    }
+    *reinterpret_cast<Codes<VEC>*>(q) = c;
+}
+
+// One row's elements of a thread: h = x + residual goes out at once, h w stays
+// in registers; sums of squares and the largest |h w| come back.
+template <typename T, int VEC>
+struct RowPart {
+    float ss = 0.f, top = 0.f;
+    __device__ __forceinline__ void add(const Pack<T, VEC>& x, const Pack<T, VEC>& r, const Pack<T, VEC>& w, bool res,
+                                        bool norm, T* sum, float (&hw)[VEC]) {
+        float h[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            h[j] = to_f32(x.v[j]);
+            if (res) h[j] += to_f32(r.v[j]);
+            ss += h[j] * h[j];
+            hw[j] = norm ? h[j] * to_f32(w.v[j]) : h[j];
+            top = max_nan(top, fabsf(hw[j]));
+        }
+        if (sum) {
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) o.v[j] = from_f32<T>(h[j]);
+            *reinterpret_cast<Pack<T, VEC>*>(sum) = o;
+        }
+    }
+    template <int LANES>
+    __device__ __forceinline__ void reduce() {  // over aligned groups of LANES lanes
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+    }
+    // over the block: one barrier, which the row's slot of shared memory is free after
+    __device__ __forceinline__ bool reduce_block(float2 (&red)[32], bool ok) {
+        const int lane = threadIdx.x & 31, n = blockDim.x >> 5;
+        reduce<32>();
+        if (lane == 0) red[threadIdx.x >> 5] = make_float2(ss, top);
+        ok = __syncthreads_and(ok);
+        const float2 v = lane < n ? red[lane] : make_float2(0.f, 0.f);
+        ss = v.x;
+        top = v.y;
+        if (n > 8) reduce<32>();
+        else reduce<8>();
+        ss = __shfl_sync(0xffffffffu, ss, 0);
+        top = __shfl_sync(0xffffffffu, top, 0);
+        return ok;
+    }
+};
+
+// What a row's elements h w are multiplied by, and its 8-bit scale.  The row's
+// factor cancels from y / scale, so a code is h w times 448 / max|h w|: three
+// roundings in all, which keeps the codes off the wrong side of a step as well
+// as a division by the scale does.  Rows near the scale's floor go through it.
+struct RowFactors {
+    float y, q, scale;
+    __device__ __forceinline__ RowFactors(const NormArgs& a, float ss, float top) {
+        y = a.w ? rsqrtf(ss * a.inv_cols + a.eps) : 1.f;
+        scale = max_nan(top * y, AMAX_FLOOR) * (1.f / Q8_MAX);
+        q = top >= AMAX_FLOOR && top * y >= AMAX_FLOOR ? __fdiv_rn(Q8_MAX, top) : y / scale;
+        if (q > 3e38f) q = 3e38f;  // zeros of such a row stay zeros
+    }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_part(const NormArgs& a, long long row, int c, const float (&hw)[VEC],
+                                           const RowFactors& f) {
+    if (a.y) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o.v[j] = from_f32<T>(hw[j] * f.y);
+        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.y) + row * a.ldy + c) = o;
+    }
+    if (a.q) store_codes<VEC>(a.q + row * a.ldq + c, hw, f.q);
+}
+
+// A row per group of G lanes, or per block (G = 0), held in registers: NV
+// vectors of VEC elements a thread.  The sum of squares and the largest |h w|
+// are reduced together, so a row is read once and a block has one barrier; the
+// largest |y| is the largest |h w| times the row's factor.
+template <typename T, int VEC, int NV, int G>
+__global__ void __launch_bounds__(G ? 256 : 1024) norm_rows_kernel(const NormArgs a) {
+    __shared__ float2 red[32];
+    const int n = G ? G : blockDim.x, tid = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
+    const long long row_ = G ? (long long)blockIdx.x * (256 / (G ? G : 1)) + threadIdx.x / (G ? G : 1) : blockIdx.x;
+    const bool live = row_ < a.rows;
+    const long long row = live ? row_ : a.rows - 1;  // lanes past the last row take part in the shuffles
+    using P = Pack<T, VEC>;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = static_cast<const T*>(a.res) + row * a.ldr;
+    P px[NV], pr[NV], pw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * n + tid) * VEC;
+        if (c < a.cols) {
+            px[i] = *reinterpret_cast<const P*>(x + c);
+            if (a.res) pr[i] = *reinterpret_cast<const P*>(r + c);
+        }
+    }
+    if (a.w) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * n + tid) * VEC;
+            if (c < a.cols) pw[i] = *reinterpret_cast<const P*>(static_cast<const T*>(a.w) + c);
+        }
+    }
+    float hw[NV][VEC];
+    RowPart<T, VEC> p;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * n + tid) * VEC;
+        if (c < a.cols)
+            p.add(px[i], pr[i], pw[i], a.res, a.w,
+                  a.sum && live ? static_cast<T*>(a.sum) + row * a.lds + c : nullptr, hw[i]);
+    }
+    if constexpr (G) p.template reduce<G>();
+    else p.reduce_block(red, true);
+    if (!live) return;
+    const RowFactors f(a, p.ss, p.top);
+    if (a.q && tid == 0) a.scale[row] = f.scale;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * n + tid) * VEC;
+        if (c < a.cols) store_part<T, VEC>(a, row, c, hw[i], f);
+    }
+}
+
+// Bulk copy global -> shared of whole 16-byte granules, completion on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// The 16-byte granules that hold a row; every granule holds at least one byte of it.
+__device__ __forceinline__ uint32_t granules(const void* row, uint32_t bytes, const char** first) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row), lo = p & ~uintptr_t(15);
+    *first = reinterpret_cast<const char*>(lo);
+    return (uint32_t)(((p + bytes + 15) & ~uintptr_t(15)) - lo);
+}
+
+constexpr int MAX_STAGES = 4;
+
+// Many rows: resident blocks walk over the rows, the next rows of x and the
+// residual on their way into a ring of `stages` slots of shared memory (a bulk
+// copy each) while one row is worked on in registers.  The copies move the
+// granules around a row, so rows may start anywhere (VEC = 1 then reads single
+// elements from shared memory).
+template <typename T, int VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+    norm_stream_kernel(const NormArgs a, int stages, uint32_t slot_bytes) {
+    extern __shared__ __align__(128) uint8_t slots[];
+    __shared__ __align__(8) uint64_t bar[MAX_STAGES];
+    __shared__ float2 red[2][32];
+    using P = Pack<T, VEC>;
+    const int n = blockDim.x, tid = threadIdx.x;
+    const long long step = gridDim.x;
+    const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
+    const uint32_t stage_bytes = slot_bytes * (a.res ? 2 : 1);
+    if (tid == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(&bar[s], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {  // one thread
+        const char *px, *pr;
+        const uint32_t nx = granules(static_cast<const T*>(a.x) + row * a.ldx, row_bytes, &px);
+        uint32_t nr = 0;
+        if (a.res) nr = granules(static_cast<const T*>(a.res) + row * a.ldr, row_bytes, &pr);
+        mbar_arrive_expect_tx(&bar[s], nx + nr);
+        bulk_load(slots + (size_t)s * stage_bytes, px, nx, &bar[s]);
+        if (a.res) bulk_load(slots + (size_t)s * stage_bytes + slot_bytes, pr, nr, &bar[s]);
+    };
+    long long row = blockIdx.x;
+    if (tid == 0)
+        for (int s = 0; s < stages; s++)
+            if (row + s * step < a.rows) load(row + s * step, s);
+    P pw[NV];
+    if (a.w) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * n + tid) * VEC;
+            if (c < a.cols) pw[i] = *reinterpret_cast<const P*>(static_cast<const T*>(a.w) + c);
+        }
+    }
+    int s = 0, flip = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (; row < a.rows; row += step) {
+        ok = mbar_wait(&bar[s], parity, &norm_err, RK_DEV_TIMEOUT_FULL);
+        const uint8_t* slot = slots + (size_t)s * stage_bytes;
+        const T* x = reinterpret_cast<const T*>(slot + (VEC == 1 ? (uint32_t)((a.xoff + row * a.ldx * sizeof(T)) & 15) : 0));
+        const T* r = reinterpret_cast<const T*>(slot + slot_bytes +
+                                                (VEC == 1 ? (uint32_t)((a.roff + row * a.ldr * sizeof(T)) & 15) : 0));
+        float hw[NV][VEC];
+        RowPart<T, VEC> p;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * n + tid) * VEC;
+            if (c < a.cols) {
+                P px = *reinterpret_cast<const P*>(x + c), pr;
+                if (a.res) pr = *reinterpret_cast<const P*>(r + c);
+                p.add(px, pr, pw[i], a.res, a.w, a.sum && ok ? static_cast<T*>(a.sum) + row * a.lds + c : nullptr, hw[i]);
+            }
+        }
+        ok = p.reduce_block(red[flip], ok);
+        flip ^= 1;
+        if (!ok) break;  // the same for the whole block
+        if (tid == 0 && row + stages * step < a.rows) load(row + stages * step, s);
+        if (++s == stages) { s = 0; parity ^= 1; }
+        const RowFactors f(a, p.ss, p.top);
+        if (a.q && tid == 0) a.scale[row] = f.scale;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * n + tid) * VEC;
+            if (c < a.cols) store_part<T, VEC>(a, row, c, hw[i], f);
+        }
+    }
+    if (!ok && tid == 0)  // a wait gave up: no copy may outlive the block
+        for (int k = 0; k < stages; k++)
+            if (row + k * step < a.rows) {
+                const int q = s + k < stages ? s + k : s + k - stages;
+                mbar_wait(&bar[q], s + k < stages ? parity : parity ^ 1, &norm_err, RK_DEV_TIMEOUT_DRAIN);
+            }
+}
+
+// Rows that do not fit one block's registers: read twice, the second time from L2.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_long_rows_kernel(const NormArgs a) {
+    __shared__ float2 red[32];
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* r = a.res ? static_cast<const T*>(a.res) + row * a.ldr : nullptr;
     const T* w = static_cast<const T*>(a.w);
-    float ss = 0.f, top = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float h = to_f32(x[c]) + (r ? to_f32(r[c]) : 0.f);
-        ss += h * h;
-        top = max_nan(top, fabsf(NORM ? h * to_f32(w[c]) : h));
-    }
-    for (int o = 16; o; o >>= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    if ((threadIdx.x & 31) == 0) { red_s[threadIdx.x >> 5] = ss; red_m[threadIdx.x >> 5] = top; }
-    __syncthreads();
-    ss = top = 0.f;
-    for (int i = 0; i < 8; i++) { ss += red_s[i]; top = max_nan(top, red_m[i]); }
-    const float inv = NORM ? rsqrtf(ss / (float)a.cols + a.eps) : 1.f;
-    const float s = max_nan(top * inv, AMAX_FLOOR) / Q8_MAX, is = 1.f / s;
-    if (a.q && threadIdx.x == 0) a.scale[row] = s;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        const float h = to_f32(x[c]) + (r ? to_f32(r[c]) : 0.f);
-        const float y = NORM ? h * inv * to_f32(w[c]) : h;
-        if (a.sum) static_cast<T*>(a.sum)[row * a.lds + c] = from_f32<T>(h);
-        if (a.y) static_cast<T*>(a.y)[row * a.ldy + c] = from_f32<T>(y);
-        if (a.q) a.q[row * a.ldq + c] = __nv_cvt_float_to_fp8(y * is, __NV_SATFINITE, __NV_E4M3);
+    using P = Pack<T, 1>;
+    RowPart<T, 1> p;
+    float hw[1];
+    for (int c = threadIdx.x; c < a.cols; c += 1024)
+        p.add(P{x[c]}, r ? P{r[c]} : P{}, w ? P{w[c]} : P{}, r, w, nullptr, hw);
+    p.reduce_block(red, true);
+    const RowFactors f(a, p.ss, p.top);
+    if (a.q && threadIdx.x == 0) a.scale[row] = f.scale;
+    RowPart<T, 1> again;
+    for (int c = threadIdx.x; c < a.cols; c += 1024) {
+        again.add(P{x[c]}, r ? P{r[c]} : P{}, w ? P{w[c]} : P{}, r, w,
+                  a.sum ? static_cast<T*>(a.sum) + row * a.lds + c : nullptr, hw);
+        store_part<T, 1>(a, row, c, hw, f);
     }
 }
 
+// columns that one block holds: 1024 threads x 32 elements
+constexpr int MAX_COLS = 32768;
+
+template <typename T, int VEC, int NV, int G>
+void launch_group(const NormArgs& a, cudaStream_t st) {
+    constexpr int per = 256 / G;
+    norm_rows_kernel<T, VEC, NV, G><<<(int)(((long long)a.rows + per - 1) / per), 256, 0, st>>>(a);
+}
+
+template <typename T, int VEC, int NV>
+void launch_block(const NormArgs& a, int vectors, cudaStream_t st) {
+    const int threads = ((vectors + NV - 1) / NV + 31) / 32 * 32;
+    norm_rows_kernel<T, VEC, NV, 0><<<a.rows, threads, 0, st>>>(a);
+}
+
+template <typename T, int VEC, int NV, int THREADS>
+cudaError_t launch_stream(const NormArgs& a, int vectors, cudaStream_t st) {
+    auto kernel = norm_stream_kernel<T, VEC, NV, THREADS>;
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    }
+    const int threads = ((vectors + NV - 1) / NV + 31) / 32 * 32;
+    const int slot = (a.cols * (int)sizeof(T) + 15) / 16 * 16 + 16, stage = slot * (a.res ? 2 : 1);
+    int ctas = 1024 / threads;  // 64 registers a thread
+    while (ctas > 1 && RING_BYTES / ctas < 2 * stage) ctas--;
+    int stages = RING_BYTES / ctas / stage;
+    stages = stages > MAX_STAGES ? MAX_STAGES : stages;
+    const long long grid = (long long)ctas * sm_count();
+    kernel<<<(int)(a.rows < grid ? a.rows : grid), threads, (size_t)stages * stage, st>>>(a, stages, (uint32_t)slot);
+    return cudaSuccess;
+}
+
+template <typename T, int VEC>
+cudaError_t launch_vec(const NormArgs& a, cudaStream_t st) {
+    const int vectors = (a.cols + VEC - 1) / VEC;
+    constexpr int E8 = VEC >= 8 ? 1 : 8 / VEC, E16 = 16 / VEC, E32 = 32 / VEC;  // vectors that make so many elements
+    if (a.cols <= 1024) {
+        const bool many = a.rows >= 8 * sm_count();
+        if (many && vectors <= 8 * E16) launch_group<T, VEC, E16, 8>(a, st);
+        else if (many && vectors <= 16 * E16) launch_group<T, VEC, E16, 16>(a, st);
+        else if (vectors <= 32 * E8) launch_group<T, VEC, E8, 32>(a, st);
+        else launch_group<T, VEC, E32, 32>(a, st);
+        return cudaSuccess;
+    }
+    const int stage = (a.cols * (int)sizeof(T) + 32) * (a.res ? 2 : 1);
+    if (a.rows > 4 * sm_count() && stage <= RING_BYTES) {
+        if (vectors <= 512 * E16) return launch_stream<T, VEC, E16, 512>(a, vectors, st);
+        if (vectors <= 1024 * E16) return launch_stream<T, VEC, E16, 1024>(a, vectors, st);
+    }
+    if (vectors <= 1024 * E8) launch_block<T, VEC, E8>(a, vectors, st);
+    else if (vectors <= 1024 * E16) launch_block<T, VEC, E16>(a, vectors, st);
+    else launch_block<T, VEC, E32>(a, vectors, st);
+    return cudaSuccess;
+}
+
 template <typename T>
-void launch(const NormArgs& a, bool norm, cudaStream_t st) {
-    if (norm) norm_rows_kernel<T, true><<<a.rows, 256, 0, st>>>(a);
-    else norm_rows_kernel<T, false><<<a.rows, 256, 0, st>>>(a);
+cudaError_t launch(const NormArgs& a, cudaStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    const bool one = a.rows == 1;
+    auto fits = [&](const void* p, long long ld, size_t e) { return aligned(p, VEC * e) && (one || ld % VEC == 0); };
+    const bool vec = a.cols % VEC == 0 && fits(a.x, a.ldx, sizeof(T)) && fits(a.w, 0, sizeof(T)) &&
+                     fits(a.res, a.ldr, sizeof(T)) && fits(a.sum, a.lds, sizeof(T)) && fits(a.y, a.ldy, sizeof(T)) &&
+                     fits(a.q, a.ldq, 1);
+    if (a.cols <= MAX_COLS) return vec ? launch_vec<T, VEC>(a, st) : launch_vec<T, 1>(a, st);
+    norm_long_rows_kernel<T><<<a.rows, 1024, 0, st>>>(a);
+    return cudaSuccess;
 }
 
 rk_status norm_rows(const NormArgs& a, bool norm, int dtype, void* stream, const char* who) {
@@ -75,16 +392,24 @@ rk_status norm_rows(const NormArgs& a, bool norm, int dtype, void* stream, const
         !aligned(a.scale, 4))
         return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (dtype) {
-        case RK_DTYPE_F32: launch<float>(a, norm, st); break;
-        case RK_DTYPE_F16: launch<__half>(a, norm, st); break;
-        default: launch<__nv_bfloat16>(a, norm, st); break;
-    }
-    const cudaError_t e2 = cudaGetLastError();
-    return e2 == cudaSuccess ? RK_OK : fail_cuda_err(RK_ERR_LAUNCH, who, e2);
+    NormArgs b = a;
+    b.inv_cols = 1.f / (float)a.cols;
+    b.xoff = (uint32_t)(reinterpret_cast<uintptr_t>(a.x) & 15);
+    b.roff = (uint32_t)(reinterpret_cast<uintptr_t>(a.res) & 15);
+    cudaError_t ce = dtype == RK_DTYPE_F32 ? launch<float>(b, st) : dtype == RK_DTYPE_F16 ? launch<__half>(b, st)
+                                                                                          : launch<__nv_bfloat16>(b, st);
+    const cudaError_t le = cudaGetLastError();
+    if (ce == cudaSuccess) ce = le;
+    return ce == cudaSuccess ? RK_OK : fail_cuda_err(RK_ERR_LAUNCH, who, ce);
 }
 
 }  // namespace
+
+void* norm_err_word() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, norm_err) == cudaSuccess ? p : nullptr;
+}
+
 }  // namespace rk
 
 using namespace rk;
