@@ -4,19 +4,11 @@
 //   y[m][n] = sum_g s[n][g] sum_{k in g} (q[n][k] - z[n][g]) x[m][k] + bias[n] + residual[m][n]
 //
 // Byte j of a weight row holds columns 2j (low half) and 2j + 1 (high half).
-#include <cooperative_groups.h>
-
 #include <atomic>
 
 #include "quant.cuh"
 #include "status.h"
 
-#ifndef Q4_TARGET
-#define Q4_TARGET 12
-#endif
-#ifndef Q4_CTAS
-#define Q4_CTAS 2
-#endif
 namespace rk {
 namespace {
 
@@ -54,9 +46,10 @@ template <> struct Q4Type<__half> { static constexpr int PARTS = 1; static const
 template <> struct Q4Type<__nv_bfloat16> { static constexpr int PARTS = 1; static constexpr bool HALF = false; };
 
 constexpr int Q4_CHUNK = 128;  // columns a warp takes at a time
-constexpr int Q4_WARPS = 8;
-// chunks of weights on their way to a warp's registers
-__host__ __device__ constexpr int q4_ahead(int nt) { return nt <= 4 ? 4 : 2; }
+
+// Warps of a block and chunks of weights on their way to a warp's registers: what 64 K registers hold.
+__host__ __device__ constexpr int q4_warps(int nt) { return nt <= 4 ? 16 : 8; }
+__host__ __device__ constexpr int q4_ahead(int nt) { return nt <= 2 ? 4 : 2; }
 
 template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -73,9 +66,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // the two codes at bits 4i and 4i + 16 of a word, less the zero point (zz: magic + z in both halves)
 template <bool HALF>
 __device__ __forceinline__ uint32_t q4_pair(uint32_t w, int i, uint32_t zz) {
-    constexpr uint32_t magic = HALF ? 0x64006400u : 0x43004300u;
-    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | magic;
-    uint32_t r;
+    const uint32_t mask = 0x000f000fu, magic = HALF ? 0x64006400u : 0x43004300u;
+    uint32_t v, r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));  // (w & mask) | magic
     if (HALF) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zz));
     else asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zz));
     return r;
@@ -84,19 +77,50 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t w, int i, uint32_t zz) {
 template <typename T>
 __device__ __forceinline__ uint16_t bits16(T v) { return *reinterpret_cast<uint16_t*>(&v); }
 
-// x = hi + mid + lo in bf16, exactly: 8 bits of the mantissa each, cut off, so that nothing overflows
-__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
+// x = hi + mid + lo in bf16, exactly: 8 bits of the mantissa each, cut off, so that nothing overflows.  Infinities and
+// NaN go whole into the first part.
+__device__ __forceinline__ void split3(float x, uint32_t (&p)[3]) {
     const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7f800000u) == 0x7f800000u) {  // infinities and NaN go whole into the first part
-        p[0] = bits16(__float2bfloat16_rn(x));
-        p[1] = p[2] = 0;
-        return;
-    }
-    const float r1 = x - __uint_as_float(u & 0xffff0000u);
+    const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+    const float r1 = finite ? x - __uint_as_float(u & 0xffff0000u) : 0.f;
     const uint32_t u1 = __float_as_uint(r1);
-    p[0] = (uint16_t)(u >> 16);
-    p[1] = (uint16_t)(u1 >> 16);
+    p[0] = u >> 16 | (!finite && (u & 0x007fffffu) ? 0x40u : 0u);
+    p[1] = u1 >> 16;
     p[2] = bits16(__float2bfloat16_rn(r1 - __uint_as_float(u1 & 0xffff0000u)));
+}
+
+// Eight columns of a row as the 16-byte blocks of their parts: the pairs (0, 4), (1, 5), (2, 6), (3, 7).
+template <typename T>
+__device__ __forceinline__ void q4_blocks(const T* x, long long left, bool vec, uint4 (&out)[Q4Type<T>::PARTS]) {
+    if constexpr (sizeof(T) == 4) {
+        float v[8];
+        if (vec && left >= 8) {
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(x);
+            *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(x + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = i < left ? x[i] : 0.f;
+        }
+        uint32_t p[8][3];
+#pragma unroll
+        for (int i = 0; i < 8; i++) split3(v[i], p[i]);
+#pragma unroll
+        for (int q = 0; q < 3; q++)
+            out[q] = make_uint4(p[0][q] | p[4][q] << 16, p[1][q] | p[5][q] << 16, p[2][q] | p[6][q] << 16,
+                                p[3][q] | p[7][q] << 16);
+    } else {
+        uint4 v;
+        if (vec && left >= 8) {
+            v = *reinterpret_cast<const uint4*>(x);
+        } else {
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = i < left ? bits16(x[i]) : 0u;
+            v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
+        out[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                            __byte_perm(v.y, v.w, 0x7632));
+    }
 }
 
 // where the 8 columns `b` of a chunk's 16 lie among its 16-byte blocks: a quad's four words side by side
@@ -107,184 +131,217 @@ __device__ __forceinline__ int q4_block(int b) {
     return b;
 }
 
-// One block: wn tiles of 16 weight rows x (8 / wn) warps that share a tile's chunks; the blocks of a cluster share
-// the chunks of their tiles.  Partial sums meet in shared memory, in a fixed order.
+// How a launch is divided, the same for all of its blocks.
+struct Q4Plan {
+    int wn;          // tiles of 16 weight rows a block works on at a time; the warps of a tile share its chunks
+    int rows;        // most weight rows of a block
+    int stage;       // chunks whose activations and scales lie in shared memory at a time
+    int pitch;       // bytes of a column's activations there, 64 mod 128: reads meet no bank twice
+    int s_pitch;     // scales of a weight row there (odd)
+    int s_off, z_off, out_off, red_off;  // shared memory: activations, scales, zero points, sums, partial sums
+    int row_block;   // first block of activation rows
+};
+
+// One block an SM, each with its share of the weight rows (as even as whole rows allow, tiles of 16 at a time, the
+// last one short) over the whole of k: every weight is read once, by one warp, and the sums never leave the block.
+// The next tiles' weights are on their way while a tile's partial sums meet in shared memory, in a fixed order.
 template <typename T, int SUB, int NT>
-__global__ void __launch_bounds__(32 * Q4_WARPS, NT <= 4 ? 2 : 1)
-    linear_q4_kernel(const Q4Args a, int wn, int stage_chunks, int row_block) {
+__global__ void __launch_bounds__(32 * q4_warps(NT), 1) linear_q4_kernel(const Q4Args a, const Q4Plan p) {
     using Ty = Q4Type<T>;
-    constexpr int PARTS = Ty::PARTS, ROWS = NT * 8 / PARTS, COLS = NT * 8;
-    constexpr int WORDS = 4 / SUB, AHEAD = q4_ahead(NT);
-    constexpr uint32_t MAGIC = Ty::HALF ? 0x64006400u : 0x43004300u;
+    constexpr int PARTS = Ty::PARTS, ROWS = NT * 8 / PARTS;
+    constexpr int WORDS = 4 / SUB, WARPS = q4_warps(NT), THREADS = 32 * WARPS, AHEAD = q4_ahead(NT);
+    constexpr uint32_t MAGIC = Ty::HALF ? 0x6400u : 0x4300u;
     extern __shared__ __align__(16) uint8_t smem[];
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wk = Q4_WARPS / wn, kw = warp / wn;
-    const int n_block = (int)(blockIdx.x / ranks) * wn * 16;
-    const int n0 = n_block + (warp % wn) * 16;
-    const long long m0 = ((long long)row_block + blockIdx.y) * ROWS;
-    const int rows = (int)(a.rows - m0 < ROWS ? a.rows - m0 : ROWS);
+    const int wn = p.wn, wk = WARPS / wn, kw = warp / wn, tile = warp % wn;
+    const int n0 = (int)((long long)a.n * blockIdx.x / gridDim.x);
+    const int n1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
+    const long long m0 = ((long long)p.row_block + blockIdx.y) * ROWS;
+    const int rows = (int)(a.rows - m0 < ROWS ? a.rows - m0 : ROWS), cols = rows * PARTS;
     const int all = (a.k + Q4_CHUNK - 1) / Q4_CHUNK;
-    const int begin = (int)((long long)all * rank / ranks), end = (int)((long long)all * (rank + 1) / ranks);
-    const int steps = (end - begin + wk - 1) / wk;       // of every warp
-    const int stage_steps = stage_chunks / wk;            // a multiple of AHEAD
-    const int pitch = stage_chunks * 256 + 64;            // bytes of a column: conflict-free 16-byte reads
     const int row_bytes = (int)(((long long)a.k + 31) / 32 * 16);
-    // rows past the last one read the last one; their sums are not stored
-    const uint8_t* wp[2];
-    size_t sp[2];
+    const int passes = (n1 - n0 + wn * 16 - 1) / (wn * 16);
+    float* out = reinterpret_cast<float*>(smem + p.out_off);
+    float* red = reinterpret_cast<float*>(smem + p.red_off);
+    const float* s_sh = reinterpret_cast<const float*>(smem + p.s_off) + (tile * 16 + g) * p.s_pitch;
+    const uint16_t* z_sh = reinterpret_cast<const uint16_t*>(smem + p.z_off) + (tile * 16 + g) * p.s_pitch;
+    // columns that no activation row fills repeat the last one
+    int xo[NT];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int n = n0 + g + 8 * i < a.n ? n0 + g + 8 * i : a.n - 1;
-        wp[i] = a.w + (long long)n * a.ldw + t * (16 / SUB);
-        sp[i] = (size_t)n * a.groups;
-    }
-    const int per = SUB == 1 ? a.group / Q4_CHUNK : 1;    // chunks a group, where a group is larger
+    for (int j = 0; j < NT; j++) xo[j] = min(j * 8 + g, cols - 1) * p.pitch + t * 16;
 
     uint32_t w[AHEAD][2][4];
-    float sc[AHEAD][2][SUB];
-    uint32_t zz[AHEAD][2][SUB];
-    auto load = [&](int step, uint32_t (&w)[2][4], float (&sc)[2][SUB], uint32_t (&zz)[2][SUB]) {
-        const int c = begin + step * wk + kw;
+    int c0 = 0, nc = min(p.stage, all);  // chunks of the stage
+    int per = (nc + wk - 1) / wk;         // of a warp and tile
+    // what to load next: chunk l_lc of the rows at l_p[]; chunks below l_full lie whole in all 16 rows
+    int l_n = 0, l_lc = 0, l_left = 0, l_full = 0;
+    const uint8_t* l_p[2];
+    auto aim = [&](int n) {
+        l_n = n;
+        l_lc = kw;
+        l_left = per;
+        l_full = n + 16 <= n1 ? min(nc, row_bytes / 64 - c0) : 0;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 2; i++) l_p[i] = a.w + (long long)(n + g + 8 * i) * a.ldw + (c0 + kw) * 64 + t * (16 / SUB);
+    };
+    auto load = [&](uint32_t (&w)[2][4]) {
+        if (l_lc < l_full) {
 #pragma unroll
-            for (int s = 0; s < SUB; s++) {
-                const int off = c * 64 + s * (64 / SUB);
-                const bool in = c < end && off + t * (16 / SUB) < row_bytes;
-                const uint8_t* p = wp[i] + off;
+            for (int i = 0; i < 2; i++) {
                 if constexpr (SUB == 1) {
-                    const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(l_p[i]));
                     w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
                 } else if constexpr (SUB == 2) {
-                    const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-                    w[i][2 * s] = v.x; w[i][2 * s + 1] = v.y;
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(l_p[i] + s * 32));
+                        w[i][2 * s] = v.x; w[i][2 * s + 1] = v.y;
+                    }
                 } else {
-                    w[i][s] = in ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+#pragma unroll
+                    for (int s = 0; s < 4; s++) w[i][s] = __ldg(reinterpret_cast<const uint32_t*>(l_p[i] + s * 16));
                 }
-                const int gi = SUB == 1 ? (per == 1 ? c : c / per) : c * SUB + s;
-                const bool gin = c < end && gi < a.groups;
-                sc[i][s] = gin ? load_as_f32(a.s, sp[i] + gi, a.s_dtype) : 0.f;
-                zz[i][s] = MAGIC + (gin && a.z ? a.z[sp[i] + gi] * 0x10001u : Q4_ZERO * 0x10001u);
             }
+        } else {  // the last rows, the last columns: a word at a time, zeros beyond them
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int left = l_lc < nc && l_n + g + 8 * i < n1 ? row_bytes - (c0 + l_lc) * 64 - t * (16 / SUB) : 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int off = j / WORDS * (64 / SUB) + j % WORDS * 4;
+                    w[i][j] = off < left ? __ldg(reinterpret_cast<const uint32_t*>(l_p[i] + off)) : 0u;
+                }
+            }
+        }
+        if (--l_left == 0) {
+            aim(l_n + wn * 16);
+        } else {
+            l_lc += wk;
+            l_p[0] += wk * 64;
+            l_p[1] += wk * 64;
         }
     };
-    float acc[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-    for (int d = 0; d < AHEAD; d++) load(d, w[d], sc[d], zz[d]);
 
-    for (int step0 = 0; step0 < steps; step0 += AHEAD) {
-        if (step0 % stage_steps == 0) {
-            // the activations of the next chunks, 8 columns at a time
-            if (step0) __syncthreads();
-            const int c0 = begin + step0 * wk, nc = min(stage_chunks, end - c0);
-            for (int u = threadIdx.x; u < rows * nc * 16; u += 32 * Q4_WARPS) {
-                const int m = u / (nc * 16), b = u - m * (nc * 16);
+    for (;;) {
+        aim(n0 + tile * 16);
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++) load(w[d]);
+        // this stage's activations and scales
+        for (int m = 0; m < rows; m++)
+            for (int b = threadIdx.x; b < nc * 16; b += THREADS) {
                 const long long col = (long long)c0 * Q4_CHUNK + b * 8;
-                const T* x = static_cast<const T*>(a.x) + (m0 + m) * a.ldx + col;
-                T v[8];
-                if (a.x_vec && col + 8 <= a.k) {
-                    struct alignas(16) Q { T v[16 / sizeof(T)]; };
+                uint4 v[PARTS];
+                q4_blocks<T>(static_cast<const T*>(a.x) + (m0 + m) * a.ldx + col, a.k - col, a.x_vec, v);
+                uint8_t* dst = smem + m * PARTS * p.pitch + ((b >> 4) * 16 + q4_block<SUB>(b & 15)) * 16;
 #pragma unroll
-                    for (int i = 0; i < 8; i += 16 / sizeof(T)) *reinterpret_cast<Q*>(v + i) = *reinterpret_cast<const Q*>(x + i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = col + i < a.k ? x[i] : from_f32<T>(0.f);
-                }
-                uint16_t p[8][3];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if constexpr (PARTS == 3) split3(v[i], p[i]);
-                    else p[i][0] = bits16(v[i]);
-                }
-                uint8_t* dst = smem + (size_t)m * PARTS * pitch + ((b >> 4) * 16 + q4_block<SUB>(b & 15)) * 16;
-#pragma unroll
-                for (int q = 0; q < PARTS; q++)
-                    *reinterpret_cast<uint4*>(dst + (size_t)q * pitch) =
-                        make_uint4(p[0][q] | (uint32_t)p[4][q] << 16, p[1][q] | (uint32_t)p[5][q] << 16,
-                                   p[2][q] | (uint32_t)p[6][q] << 16, p[3][q] | (uint32_t)p[7][q] << 16);
+                for (int q = 0; q < PARTS; q++) *reinterpret_cast<uint4*>(dst + q * p.pitch) = v[q];
             }
-            __syncthreads();
+        for (int i = warp; i < n1 - n0; i += WARPS) {
+            const size_t row = (size_t)(n0 + i) * a.groups;
+            for (int b = lane; b < nc * SUB; b += 32) {
+                const int gi = SUB == 1 ? (c0 + b) / (a.group / Q4_CHUNK) : c0 * SUB + b;
+                const size_t at = row + min(gi, a.groups - 1);  // past the last group x is zero
+                reinterpret_cast<float*>(smem + p.s_off)[i * p.s_pitch + b] = load_as_f32(a.s, at, a.s_dtype);
+                if (a.z) reinterpret_cast<uint16_t*>(smem + p.z_off)[i * p.s_pitch + b] = (uint16_t)(MAGIC + a.z[at]);
+            }
         }
+        __syncthreads();
+        float acc[NT][4];
 #pragma unroll
-        for (int d = 0; d < AHEAD; d++) {
-            const int step = step0 + d;
-            if (begin + step * wk + kw < end) {  // the same for the whole warp
-                const uint8_t* xb = smem + (size_t)g * pitch + ((step % stage_steps) * wk + kw) * 256 + t * 16;
+        for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        int pass = 0, at = 0;  // the tile and chunk worked on
+        while (pass < passes) {
 #pragma unroll
-                for (int s = 0; s < SUB; s++) {
-                    float part[NT][4];
+            for (int d = 0; d < AHEAD; d++) {
+                if (pass >= passes) break;
+                const int lc = kw + at * wk;
+                if (lc < nc) {  // the same for the whole warp
+                    const uint8_t* xb = smem + lc * 256;
+                    const int so = pass * wn * 16 * p.s_pitch + lc * SUB;
 #pragma unroll
-                    for (int j = 0; j < NT; j++) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
+                    for (int s = 0; s < SUB; s++) {
+                        const float s0 = s_sh[so + s], s1 = s_sh[so + 8 * p.s_pitch + s];
+                        uint32_t zz[2] = {(MAGIC + Q4_ZERO) * 0x10001u, (MAGIC + Q4_ZERO) * 0x10001u};
+                        if (a.z) {
+                            zz[0] = z_sh[so + s] * 0x10001u;
+                            zz[1] = z_sh[so + 8 * p.s_pitch + s] * 0x10001u;
+                        }
+                        float part[NT][4];
 #pragma unroll
-                    for (int q = s * WORDS; q < (s + 1) * WORDS; q++) {
-                        uint32_t f0[4], f1[4];
+                        for (int j = 0; j < NT; j++) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            f0[i] = q4_pair<Ty::HALF>(w[d][i][q], 0, zz[d][i][s]);
-                            f0[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 1, zz[d][i][s]);
-                            f1[i] = q4_pair<Ty::HALF>(w[d][i][q], 2, zz[d][i][s]);
-                            f1[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 3, zz[d][i][s]);
+                        for (int q = s * WORDS; q < (s + 1) * WORDS; q++) {
+                            uint32_t f0[4], f1[4];
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                f0[i] = q4_pair<Ty::HALF>(w[d][i][q], 0, zz[i]);
+                                f0[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 1, zz[i]);
+                                f1[i] = q4_pair<Ty::HALF>(w[d][i][q], 2, zz[i]);
+                                f1[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 3, zz[i]);
+                            }
+#pragma unroll
+                            for (int j = 0; j < NT; j++) {
+                                const uint4 b = *reinterpret_cast<const uint4*>(xb + xo[j] + q * 64);
+                                mma16816<Ty::HALF>(part[j], f0, b.x, b.y);
+                                mma16816<Ty::HALF>(part[j], f1, b.z, b.w);
+                            }
                         }
 #pragma unroll
                         for (int j = 0; j < NT; j++) {
-                            const uint4 b = *reinterpret_cast<const uint4*>(xb + (size_t)j * 8 * pitch + q * 64);
-                            mma16816<Ty::HALF>(part[j], f0, b.x, b.y);
-                            mma16816<Ty::HALF>(part[j], f1, b.z, b.w);
+                            acc[j][0] += s0 * part[j][0];
+                            acc[j][1] += s0 * part[j][1];
+                            acc[j][2] += s1 * part[j][2];
+                            acc[j][3] += s1 * part[j][3];
                         }
                     }
+                }
+                load(w[d]);
+                if (++at == per) {
+                    // the warps' sums of this tile: red[pass & 1][warp][16 rows][columns], added up by `rows` threads
+                    float* r = red + ((pass & 1) * WARPS + warp) * 16 * (NT * 8 + 1) + g * (NT * 8 + 1) + 2 * t;
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
-                        acc[j][0] += sc[d][0][s] * part[j][0];
-                        acc[j][1] += sc[d][0][s] * part[j][1];
-                        acc[j][2] += sc[d][1][s] * part[j][2];
-                        acc[j][3] += sc[d][1][s] * part[j][3];
+                        r[j * 8] = acc[j][0];
+                        r[j * 8 + 1] = acc[j][1];
+                        r[8 * (NT * 8 + 1) + j * 8] = acc[j][2];
+                        r[8 * (NT * 8 + 1) + j * 8 + 1] = acc[j][3];
+                        acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
                     }
+                    __syncthreads();
+                    for (int u = threadIdx.x; u < wn * 16 * rows; u += THREADS) {
+                        const int i = u % (wn * 16), m = u / (wn * 16), n = pass * wn * 16 + i;
+                        if (n < n1 - n0) {
+                            const float* rb = red + ((pass & 1) * WARPS + (i >> 4)) * 16 * (NT * 8 + 1) +
+                                              (i & 15) * (NT * 8 + 1) + m * PARTS;
+                            float v = c0 ? out[m * p.rows + n] : 0.f;
+                            for (int k = 0; k < wk; k++) {
+#pragma unroll
+                                for (int q = PARTS - 1; q >= 0; q--) v += rb[k * wn * 16 * (NT * 8 + 1) + q];
+                            }
+                            out[m * p.rows + n] = v;
+                        }
+                    }
+                    at = 0;
+                    pass++;
                 }
             }
-            load(step + AHEAD, w[d], sc[d], zz[d]);
         }
+        c0 += nc;
+        __syncthreads();
+        if (c0 >= all) break;
+        nc = min(p.stage, all - c0);
+        per = (nc + wk - 1) / wk;
     }
-
-    // partial sums: red[warp][COLS][16 rows], then over the warps of a tile, then over the cluster's blocks
-    float* red = reinterpret_cast<float*>(smem);
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        float* r = red + ((size_t)warp * COLS + j * 8 + 2 * t) * 17 + g;
-        r[0] = acc[j][0];
-        r[17] = acc[j][1];
-        r[8] = acc[j][2];
-        r[25] = acc[j][3];
-    }
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    // block `rank` finishes its share of the outputs
-    const int outs = rows * wn * 16;
-    for (int u = rank * 32 * Q4_WARPS + threadIdx.x; u < outs; u += ranks * 32 * Q4_WARPS) {
-        const int m = u / (wn * 16), i = u - m * (wn * 16);
-        const int n = n_block + i;
-        if (n >= a.n) continue;
-        float v = 0.f;
-        for (int b = 0; b < ranks; b++) {
-            const float* rb = ranks > 1 ? cluster.map_shared_rank(red, b) : red;
-#pragma unroll
-            for (int q = PARTS - 1; q >= 0; q--)
-                for (int k = 0; k < wk; k++)
-                    v += rb[((size_t)(k * wn + (i >> 4)) * COLS + m * PARTS + q) * 17 + (i & 15)];
+    for (int m = 0; m < rows; m++)
+        for (int i = threadIdx.x; i < n1 - n0; i += THREADS) {
+            float v = out[m * p.rows + i];
+            if (a.bias) v += a.bias[n0 + i];
+            if (a.res) v += to_f32(static_cast<const T*>(a.res)[(m0 + m) * a.ldr + n0 + i]);
+            static_cast<T*>(a.y)[(m0 + m) * a.ldy + n0 + i] = from_f32<T>(v);
         }
-        if (a.bias) v += a.bias[n];
-        if (a.res) v += to_f32(static_cast<const T*>(a.res)[(m0 + m) * a.ldr + n]);
-        static_cast<T*>(a.y)[(m0 + m) * a.ldy + n] = from_f32<T>(v);
-    }
-    if (ranks > 1) cluster.sync();  // no block leaves while another reads its sums
 }
 
-constexpr int Q4_SMEM = 200 * 1024;
+constexpr int Q4_SMEM = 220 * 1024;
 
 template <typename T, int SUB, int NT>
 cudaError_t launch_nt(const Q4Args& a, cudaStream_t st) {
@@ -298,43 +355,37 @@ cudaError_t launch_nt(const Q4Args& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    constexpr int PARTS = Q4Type<T>::PARTS, ROWS = NT * 8 / PARTS;
-    const int tiles = (a.n + 15) / 16, chunks = (a.k + Q4_CHUNK - 1) / Q4_CHUNK;
-    const int target = Q4_TARGET * sm_count();  // warps with work of their own
-    int wn = Q4_WARPS;
-    constexpr int AHEAD = q4_ahead(NT), COLS = NT * 8;
-    auto stage_bytes = [&](int chunks_) { return COLS * (chunks_ * 256 + 64); };
-    while (wn > 1 && (long long)tiles * (Q4_WARPS / wn) < target && Q4_WARPS / wn * 2 <= chunks &&
-           stage_bytes(Q4_WARPS / wn * 2 * AHEAD) <= Q4_SMEM)
-        wn /= 2;
-    const int wk = Q4_WARPS / wn, unit = wk * AHEAD;
-    const int groups_n = (tiles + wn - 1) / wn;
-    int ranks = 1;
-    while (ranks < 8 && (long long)groups_n * ranks * 2 <= Q4_CTAS * sm_count() && chunks >= ranks * 2 * unit) ranks *= 2;
-    // activations of `stage` chunks at a time; two blocks an SM where their registers allow it
-    const int mine = (chunks + ranks - 1) / ranks;
-    int stage = (mine + unit - 1) / unit * unit;
-    while (stage > unit && stage_bytes(stage) > (NT <= 4 ? Q4_SMEM / 2 : Q4_SMEM)) stage -= unit;
-    size_t smem = (size_t)stage_bytes(stage);
-    const size_t red = (size_t)Q4_WARPS * NT * 8 * 17 * 4;
-    if (smem < red) smem = red;
+    constexpr int PARTS = Q4Type<T>::PARTS, ROWS = NT * 8 / PARTS, WARPS = q4_warps(NT);
+    constexpr int MAX_ROWS = 512;  // weight rows of a block: their sums and scales lie in shared memory
+    const int chunks = (a.k + Q4_CHUNK - 1) / Q4_CHUNK, sms = sm_count();
+    const int m = a.rows < ROWS ? a.rows : ROWS;
+    int blocks_n = a.n < sms ? a.n : sms;
+    while ((a.n + blocks_n - 1) / blocks_n > MAX_ROWS) blocks_n += sms;
+    Q4Plan p = {};
+    p.rows = (a.n + blocks_n - 1) / blocks_n;
+    // as many warps on a tile as it has chunks for
+    p.wn = 1;
+    while (p.wn < WARPS && WARPS / p.wn > chunks) p.wn *= 2;
+    const int red = 2 * WARPS * 16 * (NT * 8 + 1) * 4;
+    const int tiles_rows = (p.rows + p.wn * 16 - 1) / (p.wn * 16) * p.wn * 16;
+    auto smem_of = [&](int stage) {
+        p.stage = stage;
+        p.pitch = stage * 256 + 64;
+        p.s_pitch = stage * SUB | 1;
+        p.s_off = m * PARTS * p.pitch;
+        p.z_off = p.s_off + tiles_rows * p.s_pitch * 4;
+        p.out_off = p.z_off + (a.z ? tiles_rows * p.s_pitch * 2 : 0);
+        p.red_off = p.out_off + m * p.rows * 4;
+        return p.red_off + red;
+    };
+    int stage = chunks < 1024 ? chunks : 1024;
+    while (stage > 1 && smem_of(stage) > Q4_SMEM) stage -= stage > 16 ? 8 : 1;
+    const int smem = smem_of(stage);
     if (smem > Q4_SMEM) return cudaErrorInvalidConfiguration;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(groups_n * ranks);
-    cfg.blockDim = dim3(32 * Q4_WARPS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const int blocks = (int)(((long long)a.rows + ROWS - 1) / ROWS);
-    for (int b = 0; b < blocks; b += 65535) {  // row blocks are the grid's second dimension
-        cfg.gridDim.y = blocks - b < 65535 ? blocks - b : 65535;
-        e = cudaLaunchKernelEx(&cfg, kernel, a, wn, stage, b);
-        if (e != cudaSuccess) return e;
+    const int blocks_m = (int)(((long long)a.rows + ROWS - 1) / ROWS);
+    for (p.row_block = 0; p.row_block < blocks_m; p.row_block += 65535) {
+        const dim3 grid(blocks_n, blocks_m - p.row_block < 65535 ? blocks_m - p.row_block : 65535);
+        kernel<<<grid, 32 * WARPS, smem, st>>>(a, p);
     }
     return cudaSuccess;
 }
