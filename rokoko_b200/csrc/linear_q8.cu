@@ -9,13 +9,10 @@
 // rows' alignment.  Operands come by TMA in K blocks of 128 bytes (the 128-byte
 // swizzle); rows and columns past the ends read as zeros.
 //
-// Two forms:
-//   tiles   one persistent block an SM, 128 x BN tiles, two accumulators, so
-//           that a tile's epilogue runs beside the next tile's products
-//   split   few tiles: the blocks of a cluster share a tile's K and add up
-//           their accumulators through each other's shared memory, in rank
-//           order; many loads in flight, the weights' bytes are the cost
-#include <cooperative_groups.h>
+// Persistent blocks, one an SM, take tiles of R <= 128 columns by C <= 256 rows
+// (any R and C: what an MMA reads beyond them only reaches accumulators that
+// nobody stores), all of K, two accumulators, so that a tile's epilogue runs
+// beside the next tile's products.  plan_tiles picks R and C.
 #include <cuda.h>
 
 #include <atomic>
@@ -37,63 +34,76 @@ struct Q8Args {
 
 __device__ uint32_t q8_err;  // set when a bounded wait of a kernel gives up
 
-constexpr int Q8_M = 128;          // weight rows of a tile
-constexpr int Q8_KB = 128;         // bytes of K a stage holds
-constexpr int Q8_W_BYTES = Q8_M * Q8_KB;
-constexpr int Q8_MAX_STAGES = 12;
-constexpr size_t Q8_SMEM = 225 * 1024;
-constexpr size_t Q8_SPLIT_SMEM = 112 * 1024;  // two blocks an SM
+constexpr int Q8_M = 128;          // the MMA's weight rows
+constexpr int Q8_KB = 128;         // bytes of K a block holds: a row of the 128-byte swizzle
+constexpr int Q8_MAX_STAGES = 32;
+constexpr int Q8_SMEM = 225 * 1024;
+constexpr int Q8_THREADS = 352;    // weights' loads, products, eight warps of epilogue, activations' loads
 
-__host__ __device__ constexpr uint32_t stage_bytes(int bn) { return Q8_W_BYTES + bn * Q8_KB; }
-
-// one output: scales, bias, residual, the one rounding
-template <typename T>
-__device__ __forceinline__ void store_out(const Q8Args& a, long long m, int n, float acc, float sx, float sw, float bias) {
-    float v = acc * (sx * sw) + bias;
-    if (a.res) v += to_f32(static_cast<const T*>(a.res)[m * a.ldr + n]);
-    static_cast<T*>(a.y)[m * a.ldy + n] = from_f32<T>(v);
-}
-
-// the MMAs of one stage
-template <int BN>
-__device__ __forceinline__ void stage_mma(uint32_t d, const uint8_t* st, bool accumulate) {
-    constexpr uint32_t idesc = umma_idesc_e4m3(Q8_M, BN);
-    const uint32_t w = smem_u32(st), x = w + Q8_W_BYTES;
-#pragma unroll
-    for (int kk = 0; kk < Q8_KB / 32; kk++)
-        umma_f8(d, sw128_kmajor_desc(w + kk * 32, 0), sw128_kmajor_desc(x + kk * 32, 0), idesc,
-                accumulate || kk > 0 ? 1u : 0u);
-}
-
-// Tiles in panels of 8 column tiles, row tiles fastest within a panel's column
-// block: the blocks at work at a time share their operands' rows in L2.
-struct Q8Tiles {
+struct Q8Plan {
+    int r, c;                // weight rows (output columns) and activation rows of a tile
+    int blocks;              // K blocks of a stage
     int n_tiles, m_tiles;
+    int stages;
+    uint32_t x_off, stage;   // bytes: the activations' place in a stage, a stage
+    uint32_t idesc;
+    uint32_t acc_cols, tmem_cols;
+    // Panels of 8 column tiles, row tiles one after the other within a panel: the blocks at work at a time share
+    // their operands' rows in L2.
     __device__ void decode(int t, int& tn, int& tm) const {
         constexpr int PANEL = 8;
-        const int per = PANEL * m_tiles, p = t / per, r = t - p * per;
+        const int per = PANEL * m_tiles, p = t / per, i = t - p * per;
         const int width = min(PANEL, n_tiles - p * PANEL);
-        tm = r / width;
-        tn = p * PANEL + r - tm * width;
+        tm = i / width;
+        tn = p * PANEL + i - tm * width;
     }
 };
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(320, 1)
-    q8_tiles_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Q8Args a,
-                    int stages) {
+// 32 rows of one output column each lane: scales, bias, residual, the one rounding
+template <typename T, bool FULL>
+__device__ __forceinline__ void store_rows(const Q8Args& a, long long m, int n, int left, const float (&acc)[32],
+                                           const float* sx, float sw, float bias) {
+    T* y = static_cast<T*>(a.y) + m * a.ldy + n;
+    T rv[32];
+    if (a.res) {
+        const T* r = static_cast<const T*>(a.res) + m * a.ldr + n;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            if (FULL || j < left) rv[j] = *r;
+            r += a.ldr;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(sx + j);
+        const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v = fmaf(acc[j + i], f[i] * sw, bias);
+            if (a.res && (FULL || j + i < left)) v += to_f32(rv[j + i]);
+            if (FULL || j + i < left) *y = from_f32<T>(v);
+            y += a.ldy;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Q8_THREADS, 1)
+    linear_q8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Q8Args a,
+                     const Q8Plan p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) uint64_t full[Q8_MAX_STAGES], empty[Q8_MAX_STAGES], acc_full[2], acc_empty[2], drain;
+    __shared__ __align__(16) float sx_sh[8][32];
     __shared__ uint32_t tmem_sh;
     __shared__ int dead;
-    constexpr uint32_t STAGE = stage_bytes(BN), COLS = 2 * BN < 32 ? 32 : 2 * BN;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kb = (a.k + Q8_KB - 1) / Q8_KB;
-    const Q8Tiles g{(a.n + Q8_M - 1) / Q8_M, (a.rows + BN - 1) / BN};
-    const int tiles = g.n_tiles * g.m_tiles;
+    const int kb = (a.k + Q8_KB - 1) / Q8_KB;  // blocks of K, and stages of them
+    const int ks = (kb + p.blocks - 1) / p.blocks;
+    const int tiles = p.n_tiles * p.m_tiles;
+    const uint32_t stages = p.stages;
     if (warp == 0 && lane == 0) {
-        for (int s = 0; s < stages; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (uint32_t s = 0; s < stages; s++) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; s++) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
         mbar_init(&drain, 1);
         dead = 0;
@@ -102,7 +112,7 @@ __global__ void __launch_bounds__(320, 1)
         tma_prefetch_desc(&tm_x);
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_sh, COLS);
+        tmem_alloc(&tmem_sh, p.tmem_cols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -110,39 +120,68 @@ __global__ void __launch_bounds__(320, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
 
-    if (warp == 0) {
-        if (lane == 0) {  // loads
-            uint32_t i = 0;
+    if (warp == 0 || warp == 10) {
+        // loads: one thread for the weights, one for the activations.  Issuing a copy and its barrier takes a thread
+        // about 200 clocks (measured, whatever the box), the products of a block as little as 264.
+        if (lane == 0) {
+            const bool w = warp == 0;
+            const CUtensorMap* map = w ? &tm_w : &tm_x;
+            const uint32_t rows = w ? p.r : p.c, off = w ? 0 : p.x_off;
+            uint32_t s = 0, parity = 1, issued = 0;
             bool alive = true;
             for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x) {
                 int tn, tm;
-                g.decode(t, tn, tm);
-                for (int b = 0; b < kb; b++, i++) {
-                    const uint32_t s = i % stages, r = i / stages;
-                    if (!mbar_wait(&empty[s], (r & 1u) ^ 1u, &q8_err, RK_DEV_TIMEOUT_EMPTY)) { alive = false; break; }
-                    uint8_t* st = ring + (size_t)s * STAGE;
-                    mbar_arrive_expect_tx(&full[s], STAGE);
-                    tma_load_2d(st, &tm_w, &full[s], b * Q8_KB, tn * Q8_M);
-                    tma_load_2d(st + Q8_W_BYTES, &tm_x, &full[s], b * Q8_KB, tm * BN);
+                p.decode(t, tn, tm);
+                const int row = w ? tn * p.r : tm * p.c;
+                for (int b = 0; b < kb; b += p.blocks) {
+                    if (!mbar_wait(&empty[s], parity, &q8_err, RK_DEV_TIMEOUT_EMPTY)) { alive = false; break; }
+                    uint8_t* st = ring + s * p.stage + off;
+                    mbar_arrive_expect_tx(&full[s], rows * Q8_KB * p.blocks);
+                    tma_load_2d(st, map, &full[s], b * Q8_KB, row);  // past the end of k: zeros
+                    if (p.blocks > 1) tma_load_2d(st + rows * Q8_KB, map, &full[s], (b + 1) * Q8_KB, row);
+                    if (issued < stages) issued++;
+                    if (++s == stages) { s = 0; parity ^= 1; }
                 }
             }
-            for (uint32_t q = i > (uint32_t)stages ? i - stages : 0u; q < i; q++)
-                mbar_wait(&full[q % stages], (q / stages) & 1u, &q8_err, RK_DEV_TIMEOUT_DRAIN);
+            // the last copy issued into each stage has landed (instant unless a consumer gave up)
+            for (uint32_t q = 0; q < issued; q++) {
+                const bool wrapped = s == 0;
+                s = wrapped ? stages - 1 : s - 1;
+                if (wrapped) parity ^= 1;
+                mbar_wait(&full[s], parity ^ 1, &q8_err, RK_DEV_TIMEOUT_DRAIN);
+            }
         }
     } else if (warp == 1) {
         if (lane == 0) {  // products
-            uint32_t i = 0, tl = 0;
+            uint32_t s = 0, parity = 0, tl = 0;
+            // descriptors count 16-byte units; shared memory ends below their 14 bits
+            const uint64_t desc = sw128_kmajor_desc(smem_u32(ring), 0);
+            const uint32_t desc0 = (uint32_t)desc, desc_hi = (uint32_t)(desc >> 32);
+            const uint32_t w_step = p.r * Q8_KB >> 4, x_step = p.c * Q8_KB >> 4;
             bool alive = true;
             for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x, tl++) {
                 const uint32_t acc = tl & 1u, ru = tl >> 1;
                 if (!mbar_wait(&acc_empty[acc], (ru & 1u) ^ 1u, &q8_err, RK_DEV_TIMEOUT_EMPTY)) break;
                 tc_fence_after();
-                for (int b = 0; b < kb; b++, i++) {
-                    const uint32_t s = i % stages, r = i / stages;
-                    if (!mbar_wait(&full[s], r & 1u, &q8_err, RK_DEV_TIMEOUT_FULL)) { alive = false; break; }
+                const uint32_t d = tmem + acc * p.acc_cols;
+                uint32_t more = 0;  // the tile's first product overwrites the accumulator
+                for (int b = 0; b < ks; b++) {
+                    if (!mbar_wait(&full[s], parity, &q8_err, RK_DEV_TIMEOUT_FULL)) { alive = false; break; }
                     tc_fence_after();
-                    stage_mma<BN>(tmem + acc * BN, ring + (size_t)s * STAGE, b > 0);
+                    const uint32_t w = desc0 + s * (p.stage >> 4), x = w + (p.x_off >> 4);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (i < p.blocks) {
+                            const uint32_t wi = w + i * w_step, xi = x + i * x_step;
+                            umma_f8(d, wi, xi, desc_hi, p.idesc, more);
+                            more = 1;
+                            umma_f8(d, wi + 2, xi + 2, desc_hi, p.idesc, 1);  // 32 bytes on
+                            umma_f8(d, wi + 4, xi + 4, desc_hi, p.idesc, 1);
+                            umma_f8(d, wi + 6, xi + 6, desc_hi, p.idesc, 1);
+                        }
+                    }
                     umma_commit(&empty[s]);
+                    if (++s == stages) { s = 0; parity ^= 1; }
                 }
                 umma_commit(&acc_full[acc]);
             }
@@ -152,37 +191,31 @@ __global__ void __launch_bounds__(320, 1)
         }
     } else {  // epilogue: lane quarter warp % 4 = 32 output columns; two warps of a quarter share the tile's rows
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float* sx_w = sx_sh[warp - 2];
         uint32_t tl = 0;
         for (int t = blockIdx.x; t < tiles; t += gridDim.x, tl++) {
             int tn, tm;
-            g.decode(t, tn, tm);
-            const int n = tn * Q8_M + quarter * 32 + lane;
-            const bool n_ok = n < a.n;
+            p.decode(t, tn, tm);
+            const int i = quarter * 32 + lane, n = tn * p.r + i;
+            const bool n_ok = i < p.r && n < a.n;
             const float sw = n_ok ? a.sw[n] : 0.f, bias = n_ok && a.bias ? a.bias[n] : 0.f;
             const uint32_t acc = tl & 1u, ru = tl >> 1;
             const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], ru & 1u, &q8_err, RK_DEV_TIMEOUT_ACC));
             tc_fence_after();
             if (!ok && lane == 0) dead = 1;
-            const uint32_t col0 = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-            const int m0 = tm * BN;
-            for (int c = half * 32; c < BN && ok; c += 64) {
-                const int left = a.rows - m0 - c;
-                if (left <= 0) break;
-                const float sx = lane < left ? a.sx[m0 + c + lane] : 0.f;
+            const uint32_t col0 = tmem + acc * p.acc_cols + ((uint32_t)(quarter * 32) << 16);
+            const long long m0 = (long long)tm * p.c;
+            const int cols = quarter * 32 < p.r && ok ? (int)min((long long)p.c, a.rows - m0) : 0;
+            for (int c = half * 32; c < cols; c += 64) {  // the same for the whole warp
+                const int left = cols - c;
+                __syncwarp();
+                sx_w[lane] = lane < left ? a.sx[m0 + c + lane] : 0.f;
                 float v[32];
                 tmem_ld32(col0 + c, v);
-                if (left >= 32) {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float s = __shfl_sync(0xffffffffu, sx, j);
-                        if (n_ok) store_out<T>(a, (long long)m0 + c + j, n, v[j], s, sw, bias);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float s = __shfl_sync(0xffffffffu, sx, j);
-                        if (n_ok && j < left) store_out<T>(a, (long long)m0 + c + j, n, v[j], s, sw, bias);
-                    }
+                __syncwarp();
+                if (n_ok) {
+                    if (left >= 32) store_rows<T, true>(a, m0 + c, n, 32, v, sx_w, sw, bias);
+                    else store_rows<T, false>(a, m0 + c, n, left, v, sx_w, sw, bias);
                 }
             }
             tc_fence_before();
@@ -196,106 +229,7 @@ __global__ void __launch_bounds__(320, 1)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, COLS);
-    }
-}
-
-// One tile per cluster; block `rank` of it sums its share of the K blocks.
-template <typename T, int BN>
-__global__ void __launch_bounds__(192)
-    q8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Q8Args a,
-                    int stages) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(8) uint64_t full[Q8_MAX_STAGES], empty[Q8_MAX_STAGES], acc_full;
-    __shared__ uint32_t tmem_sh;
-    constexpr uint32_t STAGE = stage_bytes(BN), COLS = BN < 32 ? 32 : BN;
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile = blockIdx.x / ranks, n_tiles = (a.n + Q8_M - 1) / Q8_M;
-    const int tn = tile % n_tiles, tm = tile / n_tiles;
-    const int kb = (a.k + Q8_KB - 1) / Q8_KB;
-    const int b0 = (int)((long long)kb * rank / ranks), b1 = (int)((long long)kb * (rank + 1) / ranks);
-    if (warp == 0 && lane == 0) {
-        for (int s = 0; s < stages; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(&acc_full, 1);
-        fence_mbar_init();
-    }
-    if (warp == 1) {
-        tmem_alloc(&tmem_sh, COLS);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_sh;
-    float* red = reinterpret_cast<float*>(ring);  // [BN][128], once the ring is done with
-    if (warp == 0) {
-        if (lane == 0) {
-            int i = 0;
-            for (int b = b0; b < b1; b++, i++) {
-                const int s = i % stages, r = i / stages;
-                if (!mbar_wait(&empty[s], (r & 1) ^ 1, &q8_err, RK_DEV_TIMEOUT_EMPTY)) break;
-                uint8_t* st = ring + (size_t)s * STAGE;
-                mbar_arrive_expect_tx(&full[s], STAGE);
-                tma_load_2d(st, &tm_w, &full[s], b * Q8_KB, tn * Q8_M);
-                tma_load_2d(st + Q8_W_BYTES, &tm_x, &full[s], b * Q8_KB, tm * BN);
-            }
-            for (int q = i > stages ? i - stages : 0; q < i; q++)
-                mbar_wait(&full[q % stages], (q / stages) & 1, &q8_err, RK_DEV_TIMEOUT_DRAIN);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            int i = 0;
-            for (int b = b0; b < b1; b++, i++) {
-                const int s = i % stages, r = i / stages;
-                if (!mbar_wait(&full[s], r & 1, &q8_err, RK_DEV_TIMEOUT_FULL)) break;
-                tc_fence_after();
-                stage_mma<BN>(tmem, ring + (size_t)s * STAGE, i > 0);
-                umma_commit(&empty[s]);
-            }
-            umma_commit(&acc_full);  // lands when every product above is done
-        }
-    }
-    __syncwarp();
-    // every warp: the accumulator is complete, and with it all reads of the ring
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, &q8_err, RK_DEV_TIMEOUT_ACC));
-    tc_fence_after();
-    __syncthreads();
-    const int cols = min(BN, a.rows - tm * BN);
-    if (warp >= 2) {
-        const int quarter = warp & 3;
-        const uint32_t col0 = tmem + ((uint32_t)(quarter * 32) << 16);
-        for (int c = 0; c < cols; c += 16) {
-            float v[16];
-            tmem_ld16(col0 + c, v);
-#pragma unroll
-            for (int j = 0; j < 16; j++) red[(c + j) * Q8_M + quarter * 32 + lane] = v[j];
-        }
-        tc_fence_before();
-    }
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    for (int u = threadIdx.x; u < (cols - rank + ranks - 1) / ranks * Q8_M; u += 192) {
-        const int c = u / Q8_M * ranks + rank, i = u % Q8_M;
-        const int n = tn * Q8_M + i;
-        if (n >= a.n || !ok) continue;
-        float v = 0.f;
-        if (ranks > 1) {
-            for (int b = 0; b < ranks; b++) v += cluster.map_shared_rank(red, b)[c * Q8_M + i];
-        } else {
-            v = red[c * Q8_M + i];
-        }
-        const long long m = (long long)tm * BN + c;
-        store_out<T>(a, m, n, v, a.sx[m], a.sw[n], a.bias ? a.bias[n] : 0.f);
-    }
-    if (ranks > 1) cluster.sync();  // no block leaves while another reads its sums
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        tmem_dealloc(tmem, COLS);
+        tmem_dealloc(tmem, p.tmem_cols);
     }
 }
 
@@ -347,65 +281,59 @@ struct Operands {
     long long ldx, ldw;
 };
 
-template <typename T, int BN>
-cudaError_t launch_tiles(const Operands& o, const Q8Args& a, cudaStream_t st) {
-    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
-    cudaError_t e = set_smem(q8_tiles_kernel<T, BN>, Q8_SMEM, ready);
-    if (e != cudaSuccess) return e;
-    CUtensorMap mw, mx;
-    if (!q8_map(&mw, o.w, o.ldw, a.n, a.k, Q8_M) || !q8_map(&mx, o.x, o.ldx, a.rows, a.k, BN)) return cudaErrorInvalidValue;
-    int stages = (int)((Q8_SMEM - 1024) / stage_bytes(BN));
-    if (stages > Q8_MAX_STAGES) stages = Q8_MAX_STAGES;
-    const long long tiles = ((long long)a.n + Q8_M - 1) / Q8_M * (((long long)a.rows + BN - 1) / BN);
-    if (tiles > 0x7fff0000LL) return cudaErrorInvalidValue;
-    const int grid = tiles < sm_count() ? (int)tiles : sm_count();
-    q8_tiles_kernel<T, BN><<<grid, 320, 1024 + stages * stage_bytes(BN), st>>>(mw, mx, a, stages);
-    return cudaSuccess;
-}
-
-template <typename T, int BN>
-cudaError_t launch_split(const Operands& o, const Q8Args& a, int ranks, cudaStream_t st) {
-    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
-    cudaError_t e = set_smem(q8_split_kernel<T, BN>, Q8_SPLIT_SMEM, ready);
-    if (e != cudaSuccess) return e;
-    CUtensorMap mw, mx;
-    if (!q8_map(&mw, o.w, o.ldw, a.n, a.k, Q8_M) || !q8_map(&mx, o.x, o.ldx, a.rows, a.k, BN)) return cudaErrorInvalidValue;
-    int stages = (int)((Q8_SPLIT_SMEM - 1024) / stage_bytes(BN));
-    if (stages > Q8_MAX_STAGES) stages = Q8_MAX_STAGES;
-    const int tiles = (a.n + Q8_M - 1) / Q8_M * ((a.rows + BN - 1) / BN);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * ranks);
-    cfg.blockDim = dim3(192);
-    cfg.dynamicSmemBytes = 1024 + stages * stage_bytes(BN);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, q8_split_kernel<T, BN>, mw, mx, a, stages);
+// Tile sizes: the least estimated time over R in steps of 8 and C in steps of 16.  Measured on B200, in clocks of a
+// block of K: its four MMAs take 4 max(C / 2, 66), its bytes come at about 72 a clock and SM from L2 when all SMs
+// pull, and its two copies take their threads 205 (140 with two blocks a stage).  An SM's tiles take their blocks of
+// K, or their epilogues where those are longer; the last epilogue stands alone.
+void plan_tiles(const Q8Args& a, int sms, Q8Plan& p) {
+    const int kb = (a.k + Q8_KB - 1) / Q8_KB;
+    double best = 1e300;
+    for (int r = Q8_M; r >= 8; r -= 8) {
+        const long long nt = ((long long)a.n + r - 1) / r;
+        if (r > 8 && r - 8 >= a.n) continue;
+        for (int c = 256; c >= 16; c -= 16) {
+            if (c > 16 && c - 16 >= a.rows) continue;
+            const long long mt = ((long long)a.rows + c - 1) / c, tiles = nt * mt;
+            const long long waves = (tiles + sms - 1) / sms;
+            const double mma = c > 132 ? 2.0 * c : 264.0, bytes = (r + c) * (Q8_KB / 72.0);
+            const double main = kb * (mma > bytes ? mma : bytes), epi = 600.0 + 8.0 * c;
+            const double t = waves * (main > epi ? main : epi) + (main < epi ? main : epi);
+            if (t < best * 0.999) {
+                best = t;
+                p.r = r;
+                p.c = c;
+                p.n_tiles = (int)nt;
+                p.m_tiles = (int)mt;
+            }
+        }
+    }
+    p.blocks = p.r + p.c <= 192 && kb > 1 ? 2 : 1;
+    p.idesc = umma_idesc_e4m3(Q8_M, p.c);
+    p.acc_cols = (uint32_t)(p.c + 31) / 32 * 32;
+    p.tmem_cols = 64;
+    while (p.tmem_cols < 2 * p.acc_cols) p.tmem_cols *= 2;
+    p.x_off = (uint32_t)(p.blocks * p.r * Q8_KB);    // multiples of 8 rows: 1024-byte aligned
+    p.stage = (uint32_t)(p.blocks * (p.r + p.c) * Q8_KB);
 }
 
 template <typename T>
 cudaError_t launch(const Operands& o, const Q8Args& a, cudaStream_t st) {
-    const int sms = sm_count(), kb = (a.k + Q8_KB - 1) / Q8_KB;
-    const long long nt = ((long long)a.n + Q8_M - 1) / Q8_M;
-    const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
-    const long long tiles = nt * (((long long)a.rows + bn - 1) / bn);
-    if (tiles <= sms) {
-        int ranks = 1;
-        while (ranks < 8 && tiles * ranks * 2 <= 2 * sms && kb >= ranks * 2) ranks *= 2;
-        switch (bn) {
-            case 16: return launch_split<T, 16>(o, a, ranks, st);
-            case 32: return launch_split<T, 32>(o, a, ranks, st);
-            case 64: return launch_split<T, 64>(o, a, ranks, st);
-            default: return launch_split<T, 128>(o, a, ranks, st);
-        }
-    }
-    if (a.rows <= 64) return launch_tiles<T, 64>(o, a, st);
-    if (a.rows <= 128) return launch_tiles<T, 128>(o, a, st);
-    return launch_tiles<T, 256>(o, a, st);
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
+    cudaError_t e = set_smem(linear_q8_kernel<T>, Q8_SMEM, ready);
+    if (e != cudaSuccess) return e;
+    Q8Plan p = {};
+    plan_tiles(a, sm_count(), p);
+    const long long tiles = (long long)p.n_tiles * p.m_tiles;
+    if (tiles > 0x7fff0000LL) return cudaErrorInvalidValue;
+    CUtensorMap mw, mx;
+    if (!q8_map(&mw, o.w, o.ldw, a.n, a.k, p.r) || !q8_map(&mx, o.x, o.ldx, a.rows, a.k, p.c)) return cudaErrorInvalidValue;
+    // an MMA reads 128 weight rows from a block's start, past the end of the last stage where a tile has fewer
+    const int last = (int)p.stage - (p.blocks - 1) * p.r * Q8_KB, over = Q8_M * Q8_KB > last ? Q8_M * Q8_KB - last : 0;
+    p.stages = (Q8_SMEM - 1024 - over) / (int)p.stage;
+    if (p.stages > Q8_MAX_STAGES) p.stages = Q8_MAX_STAGES;
+    const int grid = tiles < sm_count() ? (int)tiles : sm_count();
+    linear_q8_kernel<T><<<grid, Q8_THREADS, 1024 + over + p.stages * (int)p.stage, st>>>(mw, mx, a, p);
+    return cudaSuccess;
 }
 
 }  // namespace
