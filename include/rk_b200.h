@@ -181,16 +181,18 @@ RK_API rk_status rk_linear_q8(const void* x, long long ldx, const float* x_scale
  * span [min(w, 0), max(w, 0)] of the group, else scale = max|w| / 7; w must be
  * finite.
  * rk_linear_q4: y[rows][n] = x w^T + bias + residual, x and y of type dtype
- * (32-bit x keeps its precision: x is split into exact 16-bit parts), bias
- * float or NULL, residual in y's type or NULL (may be y itself).  Meant for few
+ * (32-bit x keeps its precision: x is split into 8-bit parts that hold all of
+ * it; scales below 2^90), bias float or NULL, residual in y's type or NULL (may be y itself).  Meant for few
  * rows, where the weights' bytes are the cost; any number of rows is right, and
  * beyond a few dozen rk_linear_q8 or the conv seam are faster. */
 RK_API rk_status rk_quantize_q4(const void* w, long long ldw, void* q, long long ldq, void* scales, uint8_t* zeros,
                                 int n, int k, int group, int dtype, int scale_dtype, void* stream);
 RK_API rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
                               const uint8_t* zeros, const float* bias, const void* residual, long long ldr, void* y,
-                              long long ldy, int rows, int n, int k, int group, int dtype, int scale_dtype,
-                              void* stream);
+                              long long ldy, void* workspace, size_t workspace_bytes, int rows, int n, int k,
+                              int group, int dtype, int scale_dtype, void* stream);
+/* Workspace bytes for rk_linear_q4 (device memory, 256-byte aligned; calls that can overlap need one each). */
+RK_API size_t rk_linear_q4_workspace_size(int rows, int n, int k, int group, int dtype);
 
 /* Synchronises `stream` and reports (and clears) the error words of the
  * operators above on the current device: RK_ERR_DEVICE_TIMEOUT when a bounded

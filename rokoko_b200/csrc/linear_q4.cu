@@ -4,15 +4,53 @@
 //   y[m][n] = sum_g s[n][g] sum_{k in g} (q[n][k] - z[n][g]) x[m][k] + bias[n] + residual[m][n]
 //
 // Byte j of a weight row holds columns 2j (low half) and 2j + 1 (high half).
+//
+// The product runs on tcgen05 (kind::f8f6f4) without rounding anything of x or
+// of the weights.  A code 0..15 alone in a byte is an e4m3 number already: it
+// reads q 2^-9, so a word of eight codes becomes two words of operand in three
+// instructions.  x is scaled by a power of two, the same for a row, and split
+// into e5m2 parts, each sixteen times finer than the one before: three hold
+// the 8 and 11 bits of bfloat16 and half, six the 24 of float.  The parts are
+// columns of the MMA's N side; a group's accumulators are read back, put
+// together and scaled in 32 bits, less z times the group's sum of x:
+//
+//   sum_g s (2^9 sum_p 16^-p D_p - z X_g)
+//
+// Two launches.  The first (q4_parts_kernel) lays the parts out in the
+// workspace as the second wants them in shared memory, with the sums X.  The
+// second gives each SM an even share of the weight rows, at most 128, the
+// MMA's M side; a share of at most 64 (32) rows fills the 128 with 2 (4)
+// ranges of k one below the other, whose parts are N columns of their own: an
+// MMA takes 66 clocks whatever N <= 112 is, so its rows are what must not lie
+// idle.  Some warps turn codes into operands, one thread issues the MMAs, four
+// warps add up the accumulators.  The weights' bytes are read once.
+//
+// A row with an infinity, a NaN, or magnitudes more than 2^30 apart does not fit
+// the parts; its sums are done one by one in 32 bits instead.
+#include <cuda_fp8.h>
+
 #include <atomic>
 
+#include "ptx.cuh"
 #include "quant.cuh"
 #include "status.h"
 
 namespace rk {
 namespace {
 
-constexpr int Q4_ZERO = 8;  // the zero point of weights that have none of their own
+constexpr int Q4_ZERO = 8;     // the zero point of weights that have none of their own
+constexpr int Q4_KB = 128;     // columns of a block of K: a row of the 128-byte swizzle
+constexpr int Q4_ROWS = 32;    // most activation rows of a pass over the weights
+constexpr int Q4_M = 128;      // the MMA's weight rows
+constexpr int Q4_STAGES = 8;      // most stages
+constexpr int Q4_CODES = 8;       // warps that turn codes into operands
+constexpr int Q4_SUMS = 8;        // warps that add up accumulators
+constexpr int Q4_A_BYTES = Q4_M * Q4_KB;
+constexpr int Q4_THREADS = 32 * (2 + Q4_CODES + Q4_SUMS);  // and x copies, products
+constexpr int Q4_SMEM = 220 * 1024;
+
+template <typename T> struct Q4Type { static constexpr int PARTS = 3; };
+template <> struct Q4Type<float> { static constexpr int PARTS = 6; };
 
 struct Q4Args {
     const void* x;
@@ -24,328 +62,474 @@ struct Q4Args {
     void* y;
     long long ldx, ldw, ldr, ldy;
     int rows, n, k, group, groups, s_dtype;
-    bool x_vec;  // rows of x start on 16-byte boundaries
+    bool x_vec;   // rows of x start on 16-byte boundaries
+    uint8_t* ws;  // per pass: its steps' stages, then the rows' Q4Row
 };
 
-// ---------------------------------------------------------------- the product
-//
-// Weight rows are the M = 16 side of mma.m16n8k16 and activation rows the N side, eight columns a tile.  Codes
-// become 16-bit values without a conversion: a code or'ed into the mantissa of 128 (bf16) or 1024 (half) reads
-// 128 + q, and 128 + z subtracted leaves the exact small integer q - z.  The sum over a group is scaled once, in 32
-// bits, so nothing of scale x code is rounded.  32-bit activations are three exact bf16 parts in three columns
-// whose sums are added at the end (24 bits); 16-bit ones are one column.
-//
-// The order of k within a matrix instruction is free, so a thread's fragment is whatever lies next to one another:
-// lane (g, t) reads 4 / SUB words of rows g and g + 8, the quad t = 0..3 covering one group (SUB = 1: 128 columns in
-// 16-byte loads, 2: 64 in 8-byte ones, 4: 32 in 4-byte ones).  A word's codes 0..7 come out in pairs (0, 4), (1, 5),
-// (2, 6), (3, 7), and the activations lie in shared memory in that order.
-
-template <typename T> struct Q4Type;
-template <> struct Q4Type<float> { static constexpr int PARTS = 3; static constexpr bool HALF = false; };
-template <> struct Q4Type<__half> { static constexpr int PARTS = 1; static constexpr bool HALF = true; };
-template <> struct Q4Type<__nv_bfloat16> { static constexpr int PARTS = 1; static constexpr bool HALF = false; };
-
-constexpr int Q4_CHUNK = 128;  // columns a warp takes at a time
-
-// Warps of a block and chunks of weights on their way to a warp's registers: what 64 K registers hold.
-__host__ __device__ constexpr int q4_warps(int nt) { return nt <= 4 ? 16 : 8; }
-__host__ __device__ constexpr int q4_ahead(int nt) { return nt <= 2 ? 4 : 2; }
-
-template <bool HALF>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if (HALF)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// the two codes at bits 4i and 4i + 16 of a word, less the zero point (zz: magic + z in both halves)
-template <bool HALF>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w, int i, uint32_t zz) {
-    const uint32_t mask = 0x000f000fu, magic = HALF ? 0x64006400u : 0x43004300u;
-    uint32_t v, r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));  // (w & mask) | magic
-    if (HALF) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zz));
-    else asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zz));
-    return r;
-}
-
-template <typename T>
-__device__ __forceinline__ uint16_t bits16(T v) { return *reinterpret_cast<uint16_t*>(&v); }
-
-// x = hi + mid + lo in bf16, exactly: 8 bits of the mantissa each, cut off, so that nothing overflows.  Infinities and
-// NaN go whole into the first part.
-__device__ __forceinline__ void split3(float x, uint32_t (&p)[3]) {
-    const uint32_t u = __float_as_uint(x);
-    const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-    const float r1 = finite ? x - __uint_as_float(u & 0xffff0000u) : 0.f;
-    const uint32_t u1 = __float_as_uint(r1);
-    p[0] = u >> 16 | (!finite && (u & 0x007fffffu) ? 0x40u : 0u);
-    p[1] = u1 >> 16;
-    p[2] = bits16(__float2bfloat16_rn(r1 - __uint_as_float(u1 & 0xffff0000u)));
-}
-
-// Eight columns of a row as the 16-byte blocks of their parts: the pairs (0, 4), (1, 5), (2, 6), (3, 7).
-template <typename T>
-__device__ __forceinline__ void q4_blocks(const T* x, long long left, bool vec, uint4 (&out)[Q4Type<T>::PARTS]) {
-    if constexpr (sizeof(T) == 4) {
-        float v[8];
-        if (vec && left >= 8) {
-            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(x);
-            *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(x + 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = i < left ? x[i] : 0.f;
-        }
-        uint32_t p[8][3];
-#pragma unroll
-        for (int i = 0; i < 8; i++) split3(v[i], p[i]);
-#pragma unroll
-        for (int q = 0; q < 3; q++)
-            out[q] = make_uint4(p[0][q] | p[4][q] << 16, p[1][q] | p[5][q] << 16, p[2][q] | p[6][q] << 16,
-                                p[3][q] | p[7][q] << 16);
-    } else {
-        uint4 v;
-        if (vec && left >= 8) {
-            v = *reinterpret_cast<const uint4*>(x);
-        } else {
-            uint32_t e[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) e[i] = i < left ? bits16(x[i]) : 0u;
-            v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-        }
-        out[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                            __byte_perm(v.y, v.w, 0x7632));
-    }
-}
-
-// where the 8 columns `b` of a chunk's 16 lie among its 16-byte blocks: a quad's four words side by side
-template <int SUB>
-__device__ __forceinline__ int q4_block(int b) {
-    if (SUB == 1) return (b & 3) * 4 + (b >> 2);
-    if (SUB == 2) return ((b >> 3) * 2 + (b & 1)) * 4 + ((b & 7) >> 1);
-    return b;
-}
+// What the parts of a row stand for.
+struct Q4Row {
+    float inv;  // 2^9 / the power of two that x was scaled by, as two factors
+    float inv2;
+    int odd;    // does not fit the parts
+    int pad;
+};
 
 // How a launch is divided, the same for all of its blocks.
 struct Q4Plan {
-    int wn;          // tiles of 16 weight rows a block works on at a time; the warps of a tile share its chunks
-    int rows;        // most weight rows of a block
-    int stage;       // chunks whose activations and scales lie in shared memory at a time
-    int pitch;       // bytes of a column's activations there, 64 mod 128: reads meet no bank twice
-    int s_pitch;     // scales of a weight row there (odd)
-    int s_off, z_off, out_off, red_off;  // shared memory: activations, scales, zero points, sums, partial sums
-    int row_block;   // first block of activation rows
+    int h, pad;          // ranges of k below one another, weight rows set aside for each (128 / h)
+    int share;           // most weight rows of a block
+    int steps;           // blocks of K of a range
+    int sub;             // groups of a block of K: 4, 2, 1
+    int mq;              // activation rows of a pass, in fours
+    int nc;              // N columns of a range: parts x mq, in eights
+    uint32_t x_bytes, x_stage;  // of a step: the operand rows [h * nc][128] and after them the sums [h][sub][mq]
+    int stages;
+    uint32_t s_off, stage;      // shared memory: [128][sub] scales and zero points of a stage, a stage
+    uint32_t acc_cols, tmem_cols, idesc;
+    int accs;                   // accumulators: 4 where they fit, 2
+    size_t pass_bytes;   // workspace of a pass
+    int pass0;           // first pass of this launch
 };
 
-// One block an SM, each with its share of the weight rows (as even as whole rows allow, tiles of 16 at a time, the
-// last one short) over the whole of k: every weight is read once, by one warp, and the sums never leave the block.
-// The next tiles' weights are on their way while a tile's partial sums meet in shared memory, in a fixed order.
-template <typename T, int SUB, int NT>
-__global__ void __launch_bounds__(32 * q4_warps(NT), 1) linear_q4_kernel(const Q4Args a, const Q4Plan p) {
-    using Ty = Q4Type<T>;
-    constexpr int PARTS = Ty::PARTS, ROWS = NT * 8 / PARTS;
-    constexpr int WORDS = 4 / SUB, WARPS = q4_warps(NT), THREADS = 32 * WARPS, AHEAD = q4_ahead(NT);
-    constexpr uint32_t MAGIC = Ty::HALF ? 0x6400u : 0x4300u;
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wn = p.wn, wk = WARPS / wn, kw = warp / wn, tile = warp % wn;
-    const int n0 = (int)((long long)a.n * blockIdx.x / gridDim.x);
-    const int n1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
-    const long long m0 = ((long long)p.row_block + blockIdx.y) * ROWS;
-    const int rows = (int)(a.rows - m0 < ROWS ? a.rows - m0 : ROWS), cols = rows * PARTS;
-    const int all = (a.k + Q4_CHUNK - 1) / Q4_CHUNK;
-    const int row_bytes = (int)(((long long)a.k + 31) / 32 * 16);
-    const int passes = (n1 - n0 + wn * 16 - 1) / (wn * 16);
-    float* out = reinterpret_cast<float*>(smem + p.out_off);
-    float* red = reinterpret_cast<float*>(smem + p.red_off);
-    const float* s_sh = reinterpret_cast<const float*>(smem + p.s_off) + (tile * 16 + g) * p.s_pitch;
-    const uint16_t* z_sh = reinterpret_cast<const uint16_t*>(smem + p.z_off) + (tile * 16 + g) * p.s_pitch;
-    // columns that no activation row fills repeat the last one
-    int xo[NT];
-#pragma unroll
-    for (int j = 0; j < NT; j++) xo[j] = min(j * 8 + g, cols - 1) * p.pitch + t * 16;
+// ---------------------------------------------------------------- the parts of x
 
-    uint32_t w[AHEAD][2][4];
-    int c0 = 0, nc = min(p.stage, all);  // chunks of the stage
-    int per = (nc + wk - 1) / wk;         // of a warp and tile
-    // what to load next: chunk l_lc of the rows at l_p[]; chunks below l_full lie whole in all 16 rows
-    int l_n = 0, l_lc = 0, l_left = 0, l_full = 0;
-    const uint8_t* l_p[2];
-    auto aim = [&](int n) {
-        l_n = n;
-        l_lc = kw;
-        l_left = per;
-        l_full = n + 16 <= n1 ? min(nc, row_bytes / 64 - c0) : 0;
-#pragma unroll
-        for (int i = 0; i < 2; i++) l_p[i] = a.w + (long long)(n + g + 8 * i) * a.ldw + (c0 + kw) * 64 + t * (16 / SUB);
-    };
-    auto load = [&](uint32_t (&w)[2][4]) {
-        if (l_lc < l_full) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                if constexpr (SUB == 1) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(l_p[i]));
-                    w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
-                } else if constexpr (SUB == 2) {
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(l_p[i] + s * 32));
-                        w[i][2 * s] = v.x; w[i][2 * s + 1] = v.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int s = 0; s < 4; s++) w[i][s] = __ldg(reinterpret_cast<const uint32_t*>(l_p[i] + s * 16));
-                }
-            }
-        } else {  // the last rows, the last columns: a word at a time, zeros beyond them
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int left = l_lc < nc && l_n + g + 8 * i < n1 ? row_bytes - (c0 + l_lc) * 64 - t * (16 / SUB) : 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int off = j / WORDS * (64 / SUB) + j % WORDS * 4;
-                    w[i][j] = off < left ? __ldg(reinterpret_cast<const uint32_t*>(l_p[i] + off)) : 0u;
-                }
-            }
-        }
-        if (--l_left == 0) {
-            aim(l_n + wn * 16);
-        } else {
-            l_lc += wk;
-            l_p[0] += wk * 64;
-            l_p[1] += wk * 64;
-        }
-    };
-
-    for (;;) {
-        aim(n0 + tile * 16);
-#pragma unroll
-        for (int d = 0; d < AHEAD; d++) load(w[d]);
-        // this stage's activations and scales
-        for (int m = 0; m < rows; m++)
-            for (int b = threadIdx.x; b < nc * 16; b += THREADS) {
-                const long long col = (long long)c0 * Q4_CHUNK + b * 8;
-                uint4 v[PARTS];
-                q4_blocks<T>(static_cast<const T*>(a.x) + (m0 + m) * a.ldx + col, a.k - col, a.x_vec, v);
-                uint8_t* dst = smem + m * PARTS * p.pitch + ((b >> 4) * 16 + q4_block<SUB>(b & 15)) * 16;
-#pragma unroll
-                for (int q = 0; q < PARTS; q++) *reinterpret_cast<uint4*>(dst + q * p.pitch) = v[q];
-            }
-        for (int i = warp; i < n1 - n0; i += WARPS) {
-            const size_t row = (size_t)(n0 + i) * a.groups;
-            for (int b = lane; b < nc * SUB; b += 32) {
-                const int gi = SUB == 1 ? (c0 + b) / (a.group / Q4_CHUNK) : c0 * SUB + b;
-                const size_t at = row + min(gi, a.groups - 1);  // past the last group x is zero
-                reinterpret_cast<float*>(smem + p.s_off)[i * p.s_pitch + b] = load_as_f32(a.s, at, a.s_dtype);
-                if (a.z) reinterpret_cast<uint16_t*>(smem + p.z_off)[i * p.s_pitch + b] = (uint16_t)(MAGIC + a.z[at]);
-            }
-        }
-        __syncthreads();
-        float acc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        int pass = 0, at = 0;  // the tile and chunk worked on
-        while (pass < passes) {
-#pragma unroll
-            for (int d = 0; d < AHEAD; d++) {
-                if (pass >= passes) break;
-                const int lc = kw + at * wk;
-                if (lc < nc) {  // the same for the whole warp
-                    const uint8_t* xb = smem + lc * 256;
-                    const int so = pass * wn * 16 * p.s_pitch + lc * SUB;
-#pragma unroll
-                    for (int s = 0; s < SUB; s++) {
-                        const float s0 = s_sh[so + s], s1 = s_sh[so + 8 * p.s_pitch + s];
-                        uint32_t zz[2] = {(MAGIC + Q4_ZERO) * 0x10001u, (MAGIC + Q4_ZERO) * 0x10001u};
-                        if (a.z) {
-                            zz[0] = z_sh[so + s] * 0x10001u;
-                            zz[1] = z_sh[so + 8 * p.s_pitch + s] * 0x10001u;
-                        }
-                        float part[NT][4];
-#pragma unroll
-                        for (int j = 0; j < NT; j++) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.f;
-#pragma unroll
-                        for (int q = s * WORDS; q < (s + 1) * WORDS; q++) {
-                            uint32_t f0[4], f1[4];
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                f0[i] = q4_pair<Ty::HALF>(w[d][i][q], 0, zz[i]);
-                                f0[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 1, zz[i]);
-                                f1[i] = q4_pair<Ty::HALF>(w[d][i][q], 2, zz[i]);
-                                f1[i + 2] = q4_pair<Ty::HALF>(w[d][i][q], 3, zz[i]);
-                            }
-#pragma unroll
-                            for (int j = 0; j < NT; j++) {
-                                const uint4 b = *reinterpret_cast<const uint4*>(xb + xo[j] + q * 64);
-                                mma16816<Ty::HALF>(part[j], f0, b.x, b.y);
-                                mma16816<Ty::HALF>(part[j], f1, b.z, b.w);
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            acc[j][0] += s0 * part[j][0];
-                            acc[j][1] += s0 * part[j][1];
-                            acc[j][2] += s1 * part[j][2];
-                            acc[j][3] += s1 * part[j][3];
-                        }
-                    }
-                }
-                load(w[d]);
-                if (++at == per) {
-                    // the warps' sums of this tile: red[pass & 1][warp][16 rows][columns], added up by `rows` threads
-                    float* r = red + ((pass & 1) * WARPS + warp) * 16 * (NT * 8 + 1) + g * (NT * 8 + 1) + 2 * t;
-#pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        r[j * 8] = acc[j][0];
-                        r[j * 8 + 1] = acc[j][1];
-                        r[8 * (NT * 8 + 1) + j * 8] = acc[j][2];
-                        r[8 * (NT * 8 + 1) + j * 8 + 1] = acc[j][3];
-                        acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-                    }
-                    __syncthreads();
-                    for (int u = threadIdx.x; u < wn * 16 * rows; u += THREADS) {
-                        const int i = u % (wn * 16), m = u / (wn * 16), n = pass * wn * 16 + i;
-                        if (n < n1 - n0) {
-                            const float* rb = red + ((pass & 1) * WARPS + (i >> 4)) * 16 * (NT * 8 + 1) +
-                                              (i & 15) * (NT * 8 + 1) + m * PARTS;
-                            float v = c0 ? out[m * p.rows + n] : 0.f;
-                            for (int k = 0; k < wk; k++) {
-#pragma unroll
-                                for (int q = PARTS - 1; q >= 0; q--) v += rb[k * wn * 16 * (NT * 8 + 1) + q];
-                            }
-                            out[m * p.rows + n] = v;
-                        }
-                    }
-                    at = 0;
-                    pass++;
-                }
-            }
-        }
-        c0 += nc;
-        __syncthreads();
-        if (c0 >= all) break;
-        nc = min(p.stage, all - c0);
-        per = (nc + wk - 1) / wk;
-    }
-    for (int m = 0; m < rows; m++)
-        for (int i = threadIdx.x; i < n1 - n0; i += THREADS) {
-            float v = out[m * p.rows + i];
-            if (a.bias) v += a.bias[n0 + i];
-            if (a.res) v += to_f32(static_cast<const T*>(a.res)[(m0 + m) * a.ldr + n0 + i]);
-            static_cast<T*>(a.y)[(m0 + m) * a.ldy + n0 + i] = from_f32<T>(v);
-        }
+// row, column byte -> offset in a tile of 128-byte rows in the 128-byte swizzle
+__device__ __forceinline__ uint32_t q4_swizzle(uint32_t row, uint32_t byte) {
+    return row * 128 + ((byte >> 4 ^ (row & 7)) << 4) + (byte & 15);
 }
 
-constexpr int Q4_SMEM = 220 * 1024;
+// Block (y: activation row, x: a slice of the blocks of K).  Every block looks over its whole row for the largest and
+// smallest magnitude, then writes the parts of its slice: eight columns a thread, in the order 0, 2, 4, 6, 1, 3, 5, 7
+// that the codes of a word come out in.
+template <typename T>
+__global__ void __launch_bounds__(256) q4_parts_kernel(const Q4Args a, const Q4Plan p) {
+    constexpr int PARTS = Q4Type<T>::PARTS;
+    __shared__ int sh_max[8], sh_min[8];
+    const int pass = p.pass0 + blockIdx.y / Q4_ROWS, m = blockIdx.y % Q4_ROWS;
+    const long long row = (long long)pass * Q4_ROWS + m;
+    if (row >= a.rows) return;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    uint8_t* ws = a.ws + (size_t)pass * p.pass_bytes;
+    auto load8 = [&](long long c, float (&v)[8]) {
+        struct alignas(16) Q { T v[16 / sizeof(T)]; };
+        if (a.x_vec && c + 8 <= a.k) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 16 / sizeof(T)) {
+                const Q q = *reinterpret_cast<const Q*>(x + c + i);
+#pragma unroll
+                for (int j = 0; j < 16 / (int)sizeof(T); j++) v[i + j] = to_f32(q.v[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = c + i < a.k ? to_f32(x[c + i]) : 0.f;
+        }
+    };
+    // exponents as integers order like magnitudes; zeros do not count
+    int top = 0, low = 255;
+    for (long long c = threadIdx.x * 8LL; c < a.k; c += 256 * 8) {
+        float v[8];
+        load8(c, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+            const int e = (int)(u >> 23);
+            top = max(top, e);
+            if (u) low = min(low, e);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) { sh_max[warp] = top; sh_min[warp] = low; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) { top = max(top, sh_max[i]); low = min(low, sh_min[i]); }
+    const bool odd = top == 255 || (low < 255 && low < top - 30);
+    // the largest magnitude comes to lie in [2^13, 2^14): e5m2 ends at 57344
+    const int shift = min(126, 13 - (top - 127));
+    const float scale = odd ? 0.f : __uint_as_float((uint32_t)(shift + 127) << 23);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const int back = 9 - shift;  // may pass a float's exponents: two factors
+        Q4Row r;
+        r.inv = ldexpf(1.f, back / 2);
+        r.inv2 = ldexpf(1.f, back - back / 2);
+        r.odd = odd;
+        r.pad = 0;
+        reinterpret_cast<Q4Row*>(ws + (size_t)p.steps * p.x_stage)[m] = r;
+    }
+    const int blocks = p.h * p.steps;
+    const int per = 16 / p.sub;  // threads whose columns make a group
+    // whole warps walk two blocks of K at a time, so that the sums' shuffles find every lane
+    for (int b0 = blockIdx.x * 2 + warp * 2 * gridDim.x; b0 < blocks; b0 += 16 * gridDim.x) {
+        const int b = b0 + (lane >> 4), g8 = lane & 15;
+        float v[8];
+        const long long c = (long long)b * Q4_KB + g8 * 8;
+        float sum = 0.f;
+        if (b < blocks) {
+            load8(c, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = odd ? 0.f : v[i] * scale;
+            sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
+        for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (b >= blocks) continue;
+        const int range = b / p.steps, step = b - range * p.steps;
+        uint8_t* st = ws + (size_t)step * p.x_stage;
+        if (g8 % per == 0)
+            reinterpret_cast<float*>(st + p.x_bytes)[(range * p.sub + g8 / per) * p.mq + m] = sum;
+#pragma unroll
+        for (int q = 0; q < PARTS; q++) {
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const __nv_fp8_storage_t f = __nv_cvt_float_to_fp8(v[i], __NV_SATFINITE, __NV_E5M2);
+                v[i] = (v[i] - __half2float(__half(__nv_cvt_fp8_to_halfraw(f, __NV_E5M2)))) * 16.f;
+                w[i & 1] |= (uint32_t)f << (8 * (i >> 1));
+            }
+            *reinterpret_cast<uint2*>(st + q4_swizzle(range * p.nc + q * p.mq + m, g8 * 8)) = make_uint2(w[0], w[1]);
+        }
+    }
+}
 
-template <typename T, int SUB, int NT>
-cudaError_t launch_nt(const Q4Args& a, cudaStream_t st) {
-    auto kernel = linear_q4_kernel<T, SUB, NT>;
+// ---------------------------------------------------------------- the product
+
+__device__ uint32_t q4_err;  // set when a bounded wait of the kernel gives up
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// 32 lanes x 4 columns, not waited for
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float (&v)[4]) {
+    uint32_t r[4];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = __uint_as_float(r[i]);
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[N][4]) {  // the loads above are in v after it
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) asm volatile("" : "+f"(v[i][j]));
+}
+
+// MB: activation rows that a thread has sums for; SUB: groups of a block of K
+template <typename T, int MB, int SUB>
+__global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a, const Q4Plan p) {
+    constexpr int PARTS = Q4Type<T>::PARTS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) uint64_t full[Q4_STAGES], empty[Q4_STAGES], d_full[4], d_empty[4], drain;
+    __shared__ uint32_t tmem_sh;
+    __shared__ int lost;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the same for a warp, and known to be
+    const int n0 = (int)((long long)a.n * blockIdx.x / gridDim.x), n1 = (int)((long long)a.n * (blockIdx.x + 1) / gridDim.x);
+    const int pass = p.pass0 + blockIdx.y;
+    const long long m0 = (long long)pass * Q4_ROWS;
+    const int rows = (int)(a.rows - m0 < Q4_ROWS ? a.rows - m0 : Q4_ROWS);
+    const uint8_t* ws = a.ws + (size_t)pass * p.pass_bytes;
+    const uint32_t stage = p.stage;
+    if (warp == 0 && lane == 0) {
+        // a stage is full when the x copy (its bytes) and both halves' codes are there, empty when the products and the
+        // warps of sums that look at it are done with it
+        for (int s = 0; s < p.stages; s++) { mbar_init(&full[s], 3); mbar_init(&empty[s], SUB == 1 ? 5 : 9); }
+        for (int s = 0; s < p.accs; s++) { mbar_init(&d_full[s], 1); mbar_init(&d_empty[s], 4); }
+        mbar_init(&drain, 1);
+        lost = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_sh, p.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_sh;
+    float* red = reinterpret_cast<float*>(ring);  // [sets][rows][128], once the ring is done with
+
+    if (warp == 0) {  // x: one copy a step
+        int i = 0, s = 0;
+        uint32_t parity = 1;
+        for (; i < p.steps; i++) {
+            if (!mbar_wait_warp(&empty[s], parity, &q4_err, RK_DEV_TIMEOUT_EMPTY)) { lost = 1; break; }
+            if (elect_one()) {
+                mbar_arrive_expect_tx(&full[s], p.x_stage);
+                bulk_copy(ring + s * stage + Q4_A_BYTES, ws + (size_t)i * p.x_stage, p.x_stage, &full[s]);
+            }
+            if (++s == p.stages) { s = 0; parity ^= 1; }
+        }
+        for (int q = i > p.stages ? i - p.stages : 0; q < i; q++)  // no copy outlives the block
+            mbar_wait_warp(&full[q % p.stages], q / p.stages & 1, &q4_err, RK_DEV_TIMEOUT_DRAIN);
+    } else if (warp == 1) {  // products
+        const uint64_t desc = sw128_kmajor_desc(smem_u32(ring), 0);
+        const uint32_t desc0 = (uint32_t)desc, desc_hi = (uint32_t)(desc >> 32);
+        uint32_t d = 0, d_parity = 1, parity = 0;
+        int s = 0;
+        bool alive = true;
+        for (int i = 0; i < p.steps && alive; i++) {
+            if (!mbar_wait_warp(&full[s], parity, &q4_err, RK_DEV_TIMEOUT_FULL)) { alive = false; break; }
+            const uint32_t w = desc0 + s * (stage >> 4), x = w + (Q4_A_BYTES >> 4);
+#pragma unroll
+            for (int b = 0; b < SUB; b++) {
+                if (!mbar_wait_warp(&d_empty[d], d_parity, &q4_err, RK_DEV_TIMEOUT_EMPTY)) { alive = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int e = 0; e < 4 / SUB; e++) {
+                        const int kk = b * (4 / SUB) + e;
+                        umma_f8(tmem + d * p.acc_cols, w + 2 * kk, x + 2 * kk, desc_hi, p.idesc, e > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&d_full[d]);
+                    if (b == SUB - 1) umma_commit(&empty[s]);
+                }
+                if ((int)++d == p.accs) { d = 0; d_parity ^= 1; }
+            }
+            if (++s == p.stages) { s = 0; parity ^= 1; }
+        }
+        if (!alive) lost = 1;
+        if (elect_one()) umma_commit(&drain);
+        mbar_wait_warp(&drain, 0, &q4_err, RK_DEV_TIMEOUT_DRAIN);
+        tc_fence_before();
+    } else if (warp < 2 + Q4_CODES) {
+        // Codes.  A warp takes one half (64 rows) of a step at a time, eight units of 16 bytes a lane, and the scales of
+        // those rows; as soon as a unit is laid out, its successor's load is on its way.
+        const int u = lane & 3, half = (warp & 1) * 64;
+        const int row_bytes = (int)(((long long)a.k + 31) / 32 * 16);
+        const int shift = p.h == 4 ? 5 : p.h == 2 ? 6 : 7;                       // row -> range
+        const uint8_t* src[2];                                                   // first rows of the half's two 32s
+        uint32_t there = 0;                                                      // units whose rows are there
+        int k_off[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int i = half + e * 32 + (lane >> 2), range = i >> shift;
+            src[e] = a.w + (long long)(n0 + i - range * p.pad) * a.ldw + (long long)range * p.steps * 64 + u * 16;
+            k_off[e] = range * p.steps * 64 + u * 16;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (n0 + i + 8 * j - range * p.pad < n1) there |= 1u << (e * 4 + j);
+        }
+        // what is not there stays as it is: rows that nobody stores, columns where x is zero
+        auto mask_of = [&](int step) {
+            uint32_t m = there;
+            if (k_off[0] + step * 64 >= row_bytes) m &= 0xf0u;
+            if (k_off[1] + step * 64 >= row_bytes) m &= 0x0fu;
+            return step < p.steps ? m : 0u;
+        };
+        // two rows a lane for the scales
+        const uint32_t per = a.group > Q4_KB ? a.group / Q4_KB : 1;              // blocks of K a group
+        size_t sz[2];
+        uint32_t block0[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int i = half + e * 32 + lane, range = i >> shift;
+            sz[e] = (size_t)min(n0 + i - range * p.pad, a.n - 1) * a.groups;
+            block0[e] = range * p.steps;
+        }
+        uint32_t s_raw[2][SUB], z_raw[2][SUB];
+        auto fetch = [&](int step) {                                             // converted only when they are used
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int b = 0; b < SUB; b++) {
+                    const uint32_t block = block0[e] + step;
+                    const uint32_t g = SUB == 1 && per > 1 ? block / per : block * SUB + b;
+                    const size_t at = sz[e] + min(g, a.groups - 1u);             // past the last group x is zero
+                    s_raw[e][b] = a.s_dtype == RK_DTYPE_F32 ? static_cast<const uint32_t*>(a.s)[at]
+                                                            : static_cast<const uint16_t*>(a.s)[at];
+                    z_raw[e][b] = a.z ? a.z[at] : Q4_ZERO;
+                }
+        };
+        uint4 w[8] = {};
+        auto load = [&](int j, int step, uint32_t m) {
+            if (m >> j & 1) w[j] = __ldg(reinterpret_cast<const uint4*>(src[j >> 2] + (j & 3) * 8 * a.ldw + (long long)step * 64));
+        };
+        constexpr int STRIDE = Q4_CODES / 2;
+        const int first = (warp - 2) >> 1;
+        {
+            const uint32_t m = mask_of(first);
+#pragma unroll
+            for (int j = 0; j < 8; j++) load(j, first, m);
+            fetch(first);
+        }
+        const uint32_t dst = (half + (lane >> 2)) * 128 + ((2 * u ^ (lane >> 2)) << 4);
+        int s = first % p.stages;
+        uint32_t parity = (first / p.stages & 1) ^ 1;
+        bool alive = true;
+#pragma unroll 1
+        for (int i = first; i < p.steps; i += STRIDE) {
+            const uint32_t m = mask_of(i + STRIDE);
+            alive = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &q4_err, RK_DEV_TIMEOUT_EMPTY));
+            if (!alive) break;
+            uint8_t* st = ring + s * stage;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint4 c = w[j];
+                constexpr uint32_t M = 0x0f0f0f0fu;
+                uint8_t* to = st + j * 1024;
+                // the second 16 bytes' place differs from the first's in the swizzled chunk's lowest bit
+                *reinterpret_cast<uint4*>(to + dst) = make_uint4(c.x & M, c.x >> 4 & M, c.y & M, c.y >> 4 & M);
+                *reinterpret_cast<uint4*>(to + (dst ^ 16)) = make_uint4(c.z & M, c.z >> 4 & M, c.w & M, c.w >> 4 & M);
+                load(j, i + STRIDE, m);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int b = 0; b < SUB; b++) {
+                    const uint32_t r = s_raw[e][b];
+                    const float f = a.s_dtype == RK_DTYPE_F32 ? __uint_as_float(r)
+                                    : a.s_dtype == RK_DTYPE_F16 ? __half2float(__ushort_as_half((uint16_t)r))
+                                                                : __uint_as_float(r << 16);
+                    // 2^-9 is left to the end, so the zero point comes in at 2^-9
+                    reinterpret_cast<float2*>(st + p.s_off)[(half + e * 32 + lane) * SUB + b] =
+                        make_float2(f, (float)z_raw[e][b] * (1.f / 512.f));
+                }
+            if (i + STRIDE < p.steps) fetch(i + STRIDE);
+            // Orders these plain writes before the MMAs' reads: here, where there is time, and not in the issuing thread.
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[s]);
+            s += STRIDE;
+            while (s >= p.stages) { s -= p.stages; parity ^= 1; }
+        }
+        if (!alive && lane == 0) lost = 1;
+    } else {
+        // Sums: lane i of the MMA's rows = range i / pad, weight row n0 + i % pad.  Two sets of four warps take turns at
+        // the accumulators.
+        const int quarter = warp & 3, i = quarter * 32 + lane, range = quarter * 32 / p.pad;
+        const int set = (warp - 2 - Q4_CODES) >> 2;
+        const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + range * p.nc;
+        float acc[MB];
+#pragma unroll
+        for (int m = 0; m < MB; m++) acc[m] = 0.f;
+        uint32_t d = set, d_parity = 0;
+        bool alive = true;
+        constexpr int TURN = SUB == 1 ? 2 : 1;  // steps from one to the next that this set looks at
+        int s = SUB == 1 ? set % p.stages : 0;
+        uint32_t parity = SUB == 1 ? set / p.stages & 1 : 0;
+#pragma unroll 1
+        for (int step = SUB == 1 ? set : 0; step < p.steps && alive; step += TURN) {
+            alive = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &q4_err, RK_DEV_TIMEOUT_FULL));
+            if (!alive) break;
+            const float* xs = reinterpret_cast<const float*>(ring + s * stage + Q4_A_BYTES + p.x_bytes) + range * SUB * p.mq;
+            const float2* sz = reinterpret_cast<const float2*>(ring + s * stage + p.s_off) + i * SUB;
+#pragma unroll 1
+            for (int b = SUB == 1 ? 0 : set; b < SUB; b += 2) {
+                alive = __all_sync(0xffffffffu, mbar_wait(&d_full[d], d_parity, &q4_err, RK_DEV_TIMEOUT_ACC));
+                if (!alive) break;
+                tc_fence_after();
+                const float f = sz[b].x, z = sz[b].y;
+#pragma unroll
+                for (int m = 0; m < MB; m += 4) {
+                    if (m < p.mq) {
+                        float v[PARTS][4];
+#pragma unroll
+                        for (int q = 0; q < PARTS; q++) tmem_ld4(base + d * p.acc_cols + q * p.mq + m, v[q]);
+                        const float4 x4 = *reinterpret_cast<const float4*>(xs + b * p.mq + m);
+                        const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+                        tmem_ld_wait(v);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            float t = v[PARTS - 1][j];
+#pragma unroll
+                            for (int q = PARTS - 2; q >= 0; q--) t = fmaf(t, 0.0625f, v[q][j]);
+                            acc[m + j] = fmaf(f, fmaf(-z, x[j], t), acc[m + j]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_empty[d]);
+                d += 2;
+                if ((int)d >= p.accs) { d = set; d_parity ^= 1; }
+            }
+            if (alive && lane == 0) mbar_arrive(&empty[s]);
+            s += TURN;
+            while (s >= p.stages) { s -= p.stages; parity ^= 1; }
+        }
+        if (!alive && lane == 0) lost = 1;
+        // every warp of sums has read its last accumulator: all products are done, and nothing of the ring is in use
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * Q4_SUMS) : "memory");
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+            if (alive && m < rows) red[(set * Q4_ROWS + m) * Q4_M + i] = acc[m];
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, p.tmem_cols);
+    }
+    if (lost) return;
+    const Q4Row* info = reinterpret_cast<const Q4Row*>(ws + (size_t)p.steps * p.x_stage);
+    for (int m = 0; m < rows; m++) {
+        const Q4Row r = info[m];
+        if (!r.odd) {
+            for (int i = threadIdx.x; i < n1 - n0; i += Q4_THREADS) {
+                const int n = n0 + i;
+                float v = 0.f;
+                for (int h = 0; h < p.h; h++) v += red[m * Q4_M + h * p.pad + i] + red[(Q4_ROWS + m) * Q4_M + h * p.pad + i];
+                v = v * r.inv * r.inv2;
+                if (a.bias) v += a.bias[n];
+                if (a.res) v += to_f32(static_cast<const T*>(a.res)[(m0 + m) * a.ldr + n]);
+                static_cast<T*>(a.y)[(m0 + m) * a.ldy + n] = from_f32<T>(v);
+            }
+        } else {  // a warp a weight row, one by one
+            const T* x = static_cast<const T*>(a.x) + (m0 + m) * a.ldx;
+            for (int n = n0 + warp; n < n1; n += Q4_THREADS / 32) {
+                const uint8_t* w = a.w + (long long)n * a.ldw;
+                float v = 0.f;
+                for (int k = lane; k < a.k; k += 32) {
+                    const size_t g = (size_t)n * a.groups + k / a.group;
+                    const int q = (w[k >> 1] >> (k & 1) * 4 & 15) - (a.z ? a.z[g] : Q4_ZERO);
+                    v += load_as_f32(a.s, g, a.s_dtype) * ((float)q * to_f32(x[k]));
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == 0) {
+                    if (a.bias) v += a.bias[n];
+                    if (a.res) v += to_f32(static_cast<const T*>(a.res)[(m0 + m) * a.ldr + n]);
+                    static_cast<T*>(a.y)[(m0 + m) * a.ldy + n] = from_f32<T>(v);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+int parts_of(int dtype) { return dtype == RK_DTYPE_F32 ? 6 : 3; }
+int sub_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
+
+// The widths that a pass has whatever the division: activation rows in fours, N columns of a range in eights.
+void pass_widths(int rows, int dtype, int& mq, int& nc) {
+    const int m = rows < Q4_ROWS ? rows : Q4_ROWS;
+    mq = (m + 3) / 4 * 4;
+    nc = (parts_of(dtype) * mq + 7) / 8 * 8;
+}
+
+// Workspace of a pass for a division into ranges of `steps` blocks of K.
+size_t pass_bytes(int rows, int group, int dtype, long long blocks) {
+    int mq, nc;
+    pass_widths(rows, dtype, mq, nc);
+    return (size_t)blocks * ((size_t)nc * 128 + (size_t)sub_of(group) * mq * 4) + Q4_ROWS * sizeof(Q4Row);
+}
+
+size_t workspace_bytes(int rows, int k, int group, int dtype) {
+    const long long passes = ((long long)rows + Q4_ROWS - 1) / Q4_ROWS, blocks = ((long long)k + Q4_KB - 1) / Q4_KB;
+    return (size_t)passes * ((pass_bytes(rows, group, dtype, blocks + 3) + 255) / 256 * 256);  // 4 even ranges of k
+}
+
+template <typename T, int MB, int SUB>
+cudaError_t launch_mb(const Q4Args& a, cudaStream_t st) {
+    auto kernel = linear_q4_kernel<T, MB, SUB>;
+    Q4Plan p = {};
     static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -355,56 +539,57 @@ cudaError_t launch_nt(const Q4Args& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    constexpr int PARTS = Q4Type<T>::PARTS, ROWS = NT * 8 / PARTS, WARPS = q4_warps(NT);
-    constexpr int MAX_ROWS = 512;  // weight rows of a block: their sums and scales lie in shared memory
-    const int chunks = (a.k + Q4_CHUNK - 1) / Q4_CHUNK, sms = sm_count();
-    const int m = a.rows < ROWS ? a.rows : ROWS;
-    int blocks_n = a.n < sms ? a.n : sms;
-    while ((a.n + blocks_n - 1) / blocks_n > MAX_ROWS) blocks_n += sms;
-    Q4Plan p = {};
-    p.rows = (a.n + blocks_n - 1) / blocks_n;
-    // as many warps on a tile as it has chunks for
-    p.wn = 1;
-    while (p.wn < WARPS && WARPS / p.wn > chunks) p.wn *= 2;
-    const int red = 2 * WARPS * 16 * (NT * 8 + 1) * 4;
-    const int tiles_rows = (p.rows + p.wn * 16 - 1) / (p.wn * 16) * p.wn * 16;
-    auto smem_of = [&](int stage) {
-        p.stage = stage;
-        p.pitch = stage * 256 + 64;
-        p.s_pitch = stage * SUB | 1;
-        p.s_off = m * PARTS * p.pitch;
-        p.z_off = p.s_off + tiles_rows * p.s_pitch * 4;
-        p.out_off = p.z_off + (a.z ? tiles_rows * p.s_pitch * 2 : 0);
-        p.red_off = p.out_off + m * p.rows * 4;
-        return p.red_off + red;
-    };
-    int stage = chunks < 1024 ? chunks : 1024;
-    while (stage > 1 && smem_of(stage) > Q4_SMEM) stage -= stage > 16 ? 8 : 1;
-    const int smem = smem_of(stage);
-    if (smem > Q4_SMEM) return cudaErrorInvalidConfiguration;
-    const int blocks_m = (int)(((long long)a.rows + ROWS - 1) / ROWS);
-    for (p.row_block = 0; p.row_block < blocks_m; p.row_block += 65535) {
-        const dim3 grid(blocks_n, blocks_m - p.row_block < 65535 ? blocks_m - p.row_block : 65535);
-        kernel<<<grid, 32 * WARPS, smem, st>>>(a, p);
+    const int sms = sm_count(), blocks = (int)(((long long)a.k + Q4_KB - 1) / Q4_KB);
+    // an even share of the weight rows for each SM, in as many rounds as 128 rows a block make it
+    long long grid = sms;
+    while ((a.n + grid - 1) / grid > Q4_M) grid += sms;
+    if (grid > a.n) grid = a.n;
+    p.share = (int)((a.n + grid - 1) / grid);
+    p.h = p.share <= 32 ? 4 : p.share <= 64 ? 2 : 1;
+    while (p.h > blocks) p.h /= 2;
+    pass_widths(a.rows, sizeof(T) == 4 ? RK_DTYPE_F32 : RK_DTYPE_F16, p.mq, p.nc);
+    while (p.h > 1 && p.h * p.nc > 128) p.h /= 2;  // wide ones need no filling: their MMAs take as long as their N
+    p.pad = Q4_M / p.h;
+    p.steps = (blocks + p.h - 1) / p.h;
+    p.sub = SUB;
+    p.x_bytes = (uint32_t)(p.h * p.nc * 128);
+    p.x_stage = p.x_bytes + (uint32_t)(p.h * p.sub * p.mq * 4);
+    const int nn = (p.h * p.nc + 15) / 16 * 16;
+    p.idesc = umma_idesc_e4m3(Q4_M, nn) | 1u << 10;  // B in e5m2
+    p.acc_cols = (uint32_t)(nn + 31) / 32 * 32;
+    p.accs = 4 * p.acc_cols <= 512 ? 4 : 2;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < p.accs * p.acc_cols) p.tmem_cols *= 2;
+    p.pass_bytes = ((size_t)p.steps * p.x_stage + Q4_ROWS * sizeof(Q4Row) + 255) / 256 * 256;
+    // an MMA of N in sixteens may read eight rows past a stage's operand rows, which the scales' place makes up for
+    p.s_off = Q4_A_BYTES + (p.x_stage + 127) / 128 * 128;
+    p.stage = (p.s_off + Q4_M * p.sub * (uint32_t)sizeof(float2) + 1023) / 1024 * 1024;
+    p.stages = (Q4_SMEM - 1024) / (int)p.stage;
+    if (p.stages > Q4_STAGES) p.stages = Q4_STAGES;
+    // A warp of codes goes on Q4_CODES / 2 steps at a time.  With fewer stages it could be two rounds ahead of a stage's
+    // barrier, whose parity would let it through.
+    if (p.stages < Q4_CODES / 2) return cudaErrorInvalidConfiguration;
+    int smem = p.stages * (int)p.stage;
+    const int red = 2 * Q4_ROWS * Q4_M * 4;
+    if (smem < red) smem = red;
+    smem += 1024;
+    const int passes = (int)(((long long)a.rows + Q4_ROWS - 1) / Q4_ROWS);
+    for (p.pass0 = 0; p.pass0 < passes; p.pass0 += 2047) {  // rows and passes are the grids' second dimension
+        const int n = passes - p.pass0 < 2047 ? passes - p.pass0 : 2047;
+        const int rows = n > 1 ? n * Q4_ROWS : (a.rows - p.pass0 * Q4_ROWS < Q4_ROWS ? a.rows - p.pass0 * Q4_ROWS : Q4_ROWS);
+        const int slices = (p.h * p.steps + 15) / 16;  // 16 blocks of K a block: two a warp
+        q4_parts_kernel<T><<<dim3(slices, rows), 256, 0, st>>>(a, p);
+        kernel<<<dim3((unsigned)grid, n), Q4_THREADS, smem, st>>>(a, p);
     }
     return cudaSuccess;
 }
 
 template <typename T, int SUB>
 cudaError_t launch_sub(const Q4Args& a, cudaStream_t st) {
-    if constexpr (Q4Type<T>::PARTS == 3) {
-        if (a.rows <= 2) return launch_nt<T, SUB, 1>(a, st);
-        if (a.rows <= 5) return launch_nt<T, SUB, 2>(a, st);
-        if (a.rows <= 8) return launch_nt<T, SUB, 3>(a, st);
-        if (a.rows <= 16) return launch_nt<T, SUB, 6>(a, st);
-        if (a.rows <= 24) return launch_nt<T, SUB, 9>(a, st);
-        return launch_nt<T, SUB, 12>(a, st);
-    } else {
-        if (a.rows <= 8) return launch_nt<T, SUB, 1>(a, st);
-        if (a.rows <= 16) return launch_nt<T, SUB, 2>(a, st);
-        if (a.rows <= 32) return launch_nt<T, SUB, 4>(a, st);
-        return launch_nt<T, SUB, 8>(a, st);
-    }
+    if (a.rows <= 4) return launch_mb<T, 4, SUB>(a, st);
+    if (a.rows <= 8) return launch_mb<T, 8, SUB>(a, st);
+    if (a.rows <= 16) return launch_mb<T, 16, SUB>(a, st);
+    return launch_mb<T, 32, SUB>(a, st);
 }
 
 template <typename T>
@@ -482,14 +667,25 @@ __global__ void __launch_bounds__(256)
 bool group_ok(int group) { return group == 32 || group == 64 || (group >= 128 && group % 128 == 0); }
 
 }  // namespace
+
+void* q4_err_word() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, q4_err) == cudaSuccess ? p : nullptr;
+}
+
 }  // namespace rk
 
 using namespace rk;
 
+extern "C" size_t rk_linear_q4_workspace_size(int rows, int n, int k, int group, int dtype) {
+    if (rows < 0 || n < 1 || k < 1 || !group_ok(group) || !dtype_ok(dtype)) return 0;
+    return rows ? workspace_bytes(rows, k, group, dtype) : 0;
+}
+
 extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
                                   const uint8_t* zeros, const float* bias, const void* residual, long long ldr,
-                                  void* y, long long ldy, int rows, int n, int k, int group, int dtype,
-                                  int scale_dtype, void* stream) {
+                                  void* y, long long ldy, void* workspace, size_t workspace_size, int rows, int n,
+                                  int k, int group, int dtype, int scale_dtype, void* stream) {
     const char* who = "rk_linear_q4: unsupported arguments";
     if (!dtype_ok(dtype) || !dtype_ok(scale_dtype) || rows < 0 || n < 1 || k < 1) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     if (!group_ok(group))
@@ -504,9 +700,11 @@ extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, l
     if (!aligned(w, 16) || (n > 1 && (ldw % 16 || ldw < row_bytes)))
         return fail(RK_ERR_CANNOT_IMPLEMENT,
                     "rk_linear_q4: weight rows hold ceil(k / 32) x 16 bytes and start on 16-byte boundaries");
+    if (!workspace || workspace_size < workspace_bytes(rows, k, group, dtype) || !aligned(workspace, 256))
+        return fail(RK_ERR_WORKSPACE, "rk_linear_q4: workspace too small or not 256-byte aligned");
     Q4Args a{x, static_cast<const uint8_t*>(w), scales, zeros, bias, residual, y, ldx, ldw, ldr, ldy, rows, n, k,
              group, (int)(((long long)k + group - 1) / group), scale_dtype,
-             aligned(x, 16) && (rows == 1 || ldx * (long long)e % 16 == 0)};
+             aligned(x, 16) && (rows == 1 || ldx * (long long)e % 16 == 0), static_cast<uint8_t*>(workspace)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t ce = dtype == RK_DTYPE_F32 ? launch<float>(a, st) : dtype == RK_DTYPE_F16 ? launch<__half>(a, st)
                                                                                           : launch<__nv_bfloat16>(a, st);

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(Q8_THREADS, 1)
     __shared__ __align__(8) uint64_t full[Q8_MAX_STAGES], empty[Q8_MAX_STAGES], acc_full[2], acc_empty[2], drain;
     __shared__ __align__(16) float sx_sh[Q8_EPI][32];
     __shared__ uint32_t tmem_sh;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the same for a warp, and known to be
     const int kb = (a.k + Q8_KB - 1) / Q8_KB;  // blocks of K, and stages of them
     const int ks = (kb + p.blocks - 1) / p.blocks;
     const int tiles = p.n_tiles * p.m_tiles;
@@ -120,74 +120,73 @@ __global__ void __launch_bounds__(Q8_THREADS, 1)
     const uint32_t tmem = tmem_sh;
 
     if (warp == 0 || warp == 2 + Q8_EPI) {
-        // loads: one thread for the weights, one for the activations.  Issuing a copy and its barrier takes a thread
-        // about 200 clocks (measured, whatever the box), the products of a block as little as 264.
-        if (lane == 0) {
-            const bool w = warp == 0;
-            const CUtensorMap* map = w ? &tm_w : &tm_x;
-            const uint32_t rows = w ? p.r : p.c, off = w ? 0 : p.x_off;
-            uint32_t s = 0, parity = 1, issued = 0;
-            bool alive = true;
-            for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x) {
-                int tn, tm;
-                p.decode(t, tn, tm);
-                const int row = w ? tn * p.r : tm * p.c;
-                for (int b = 0; b < kb; b += p.blocks) {
-                    if (!mbar_wait(&empty[s], parity, &q8_err, RK_DEV_TIMEOUT_EMPTY)) { alive = false; break; }
-                    uint8_t* st = ring + s * p.stage + off;
+        // loads: one warp for the weights, one for the activations; issuing copies is what bounds narrow tiles
+        const bool w = warp == 0;
+        const CUtensorMap* map = w ? &tm_w : &tm_x;
+        const uint32_t rows = w ? p.r : p.c, off = w ? 0 : p.x_off;
+        uint32_t s = 0, parity = 1, issued = 0;
+        bool alive = true;
+        for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x) {
+            int tn, tm;
+            p.decode(t, tn, tm);
+            const int row = w ? tn * p.r : tm * p.c;
+            for (int b = 0; b < kb; b += p.blocks) {
+                if (!mbar_wait_warp(&empty[s], parity, &q8_err, RK_DEV_TIMEOUT_EMPTY)) { alive = false; break; }
+                uint8_t* st = ring + s * p.stage + off;
+                if (elect_one()) {
                     mbar_arrive_expect_tx(&full[s], rows * Q8_KB * p.blocks);
                     tma_load_2d(st, map, &full[s], b * Q8_KB, row);  // past the end of k: zeros
                     if (p.blocks > 1) tma_load_2d(st + rows * Q8_KB, map, &full[s], (b + 1) * Q8_KB, row);
-                    if (issued < stages) issued++;
-                    if (++s == stages) { s = 0; parity ^= 1; }
                 }
-            }
-            // the last copy issued into each stage has landed (instant unless a consumer gave up)
-            for (uint32_t q = 0; q < issued; q++) {
-                const bool wrapped = s == 0;
-                s = wrapped ? stages - 1 : s - 1;
-                if (wrapped) parity ^= 1;
-                mbar_wait(&full[s], parity ^ 1, &q8_err, RK_DEV_TIMEOUT_DRAIN);
+                if (issued < stages) issued++;
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // products
-            uint32_t s = 0, parity = 0, tl = 0;
-            // descriptors count 16-byte units; shared memory ends below their 14 bits
-            const uint64_t desc = sw128_kmajor_desc(smem_u32(ring), 0);
-            const uint32_t desc0 = (uint32_t)desc, desc_hi = (uint32_t)(desc >> 32);
-            const uint32_t w_step = p.r * Q8_KB >> 4, x_step = p.c * Q8_KB >> 4;
-            bool alive = true;
-            for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x, tl++) {
-                const uint32_t acc = tl & 1u, ru = tl >> 1;
-                if (!mbar_wait(&acc_empty[acc], (ru & 1u) ^ 1u, &q8_err, RK_DEV_TIMEOUT_EMPTY)) break;
+        // the last copy issued into each stage has landed (instant unless a consumer gave up)
+        for (uint32_t q = 0; q < issued; q++) {
+            const bool wrapped = s == 0;
+            s = wrapped ? stages - 1 : s - 1;
+            if (wrapped) parity ^= 1;
+            mbar_wait_warp(&full[s], parity ^ 1, &q8_err, RK_DEV_TIMEOUT_DRAIN);
+        }
+    } else if (warp == 1) {  // products
+        uint32_t s = 0, parity = 0, tl = 0;
+        // descriptors count 16-byte units; shared memory ends below their 14 bits
+        const uint64_t desc = sw128_kmajor_desc(smem_u32(ring), 0);
+        const uint32_t desc0 = (uint32_t)desc, desc_hi = (uint32_t)(desc >> 32);
+        const uint32_t w_step = p.r * Q8_KB >> 4, x_step = p.c * Q8_KB >> 4;
+        bool alive = true;
+        for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x, tl++) {
+            const uint32_t acc = tl & 1u, ru = tl >> 1;
+            if (!mbar_wait_warp(&acc_empty[acc], (ru & 1u) ^ 1u, &q8_err, RK_DEV_TIMEOUT_EMPTY)) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * p.acc_cols;
+            uint32_t more = 0;  // the tile's first product overwrites the accumulator
+            for (int b = 0; b < ks; b++) {
+                if (!mbar_wait_warp(&full[s], parity, &q8_err, RK_DEV_TIMEOUT_FULL)) { alive = false; break; }
                 tc_fence_after();
-                const uint32_t d = tmem + acc * p.acc_cols;
-                uint32_t more = 0;  // the tile's first product overwrites the accumulator
-                for (int b = 0; b < ks; b++) {
-                    if (!mbar_wait(&full[s], parity, &q8_err, RK_DEV_TIMEOUT_FULL)) { alive = false; break; }
-                    tc_fence_after();
-                    const uint32_t w = desc0 + s * (p.stage >> 4), x = w + (p.x_off >> 4);
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        if (i < p.blocks) {
-                            const uint32_t wi = w + i * w_step, xi = x + i * x_step;
-                            umma_f8(d, wi, xi, desc_hi, p.idesc, more);
-                            more = 1;
-                            umma_f8(d, wi + 2, xi + 2, desc_hi, p.idesc, 1);  // 32 bytes on
-                            umma_f8(d, wi + 4, xi + 4, desc_hi, p.idesc, 1);
-                            umma_f8(d, wi + 6, xi + 6, desc_hi, p.idesc, 1);
-                        }
+                const uint32_t w = desc0 + s * (p.stage >> 4), x = w + (p.x_off >> 4);
+                if (elect_one()) {
+                    umma_f8(d, w, x, desc_hi, p.idesc, more);
+                    umma_f8(d, w + 2, x + 2, desc_hi, p.idesc, 1);  // 32 bytes on
+                    umma_f8(d, w + 4, x + 4, desc_hi, p.idesc, 1);
+                    umma_f8(d, w + 6, x + 6, desc_hi, p.idesc, 1);
+                    if (p.blocks > 1) {
+                        umma_f8(d, w + w_step, x + x_step, desc_hi, p.idesc, 1);
+                        umma_f8(d, w + w_step + 2, x + x_step + 2, desc_hi, p.idesc, 1);
+                        umma_f8(d, w + w_step + 4, x + x_step + 4, desc_hi, p.idesc, 1);
+                        umma_f8(d, w + w_step + 6, x + x_step + 6, desc_hi, p.idesc, 1);
                     }
                     umma_commit(&empty[s]);
-                    if (++s == stages) { s = 0; parity ^= 1; }
                 }
-                umma_commit(&acc_full[acc]);
+                more = 1;
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
-            umma_commit(&drain);
-            mbar_wait(&drain, 0, &q8_err, RK_DEV_TIMEOUT_DRAIN);
-            tc_fence_before();
+            if (elect_one()) umma_commit(&acc_full[acc]);
         }
+        if (elect_one()) umma_commit(&drain);
+        mbar_wait_warp(&drain, 0, &q8_err, RK_DEV_TIMEOUT_DRAIN);
+        tc_fence_before();
     } else {  // epilogue: lane quarter warp % 4 = 32 output columns; the warps of a quarter share the tile's rows
         constexpr int SHARE = Q8_EPI / 4, CHUNKS = 8 / SHARE;
         const int quarter = warp & 3, part = (warp - 2) >> 2;

@@ -25,7 +25,7 @@ int sm_count() {
 
 extern "C" rk_status rk_linear_check(void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    void* words[] = {rk::norm_err_word(), rk::q8_err_word()};
+    void* words[] = {rk::norm_err_word(), rk::q8_err_word(), rk::q4_err_word()};
     uint32_t seen = 0;
     for (void* p : words) {
         uint32_t e = 0;

@@ -46,6 +46,7 @@ int sm_count();
 // Device addresses of the error words of the operators' bounded waits, on the current device.
 void* norm_err_word();
 void* q8_err_word();
+void* q4_err_word();
 
 inline size_t dtype_bytes(int dtype) { return dtype == RK_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == RK_DTYPE_F32 || dtype == RK_DTYPE_F16 || dtype == RK_DTYPE_BF16; }

@@ -68,7 +68,8 @@ SIGNATURES = [
      [_p, _ll, _p, _p, _ll, _p, _p, _p, _ll, _p, _ll] + [ctypes.c_int] * 4 + [_p]),
     ("rk_quantize_q4", ctypes.c_int, [_p, _ll, _p, _ll, _p, _p] + [ctypes.c_int] * 5 + [_p]),
     ("rk_linear_q4", ctypes.c_int,
-     [_p, _ll, _p, _ll, _p, _p, _p, _p, _ll, _p, _ll] + [ctypes.c_int] * 6 + [_p]),
+     [_p, _ll, _p, _ll, _p, _p, _p, _p, _ll, _p, _ll, _p, ctypes.c_size_t] + [ctypes.c_int] * 6 + [_p]),
+    ("rk_linear_q4_workspace_size", ctypes.c_size_t, [ctypes.c_int] * 5),
     ("rk_linear_check", ctypes.c_int, [_p]),
     ("rk_create", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(rk_options), ctypes.POINTER(ctypes.c_void_p)]),
     ("rk_destroy", None, [ctypes.c_void_p]),

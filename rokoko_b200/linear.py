@@ -266,8 +266,10 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
             raise ValueError("zeros: a contiguous tensor is expected")
         zp = zeros.data_ptr()
     out, tail = _finish_args(x, rows, n, dtype, dev, bias, residual, out)
-    _call("rk_linear_q4", dev, x.data_ptr(), ldx, pw, ldw, scales.data_ptr(), zp, *tail, rows, n, k, group, dt,
-          st)
+    size = lib.load().rk_linear_q4_workspace_size(rows, n, k, group, dt)
+    ws = x.new_empty((size,), dtype=torch.uint8)  # torch's blocks start on 512-byte boundaries
+    _call("rk_linear_q4", dev, x.data_ptr(), ldx, pw, ldw, scales.data_ptr(), zp, *tail, ws.data_ptr(), size, rows, n, k,
+          group, dt, st)
     return out
 
 

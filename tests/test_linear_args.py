@@ -57,8 +57,8 @@ def test_linear_q8_refuses(rk_lib, bad):
 
 
 def _q4(L, x=P, ldx=96, w=P, ldw=48, s=P, z=None, b=None, r=None, ldr=0, y=P, ldy=32, rows=4, n=32, k=96, group=32,
-        dtype=F32, sdtype=F32):
-    return L.rk_linear_q4(x, ldx, w, ldw, s, z, b, r, ldr, y, ldy, rows, n, k, group, dtype, sdtype, None)
+        dtype=F32, sdtype=F32, ws=P, size=1 << 40):
+    return L.rk_linear_q4(x, ldx, w, ldw, s, z, b, r, ldr, y, ldy, ws, size, rows, n, k, group, dtype, sdtype, None)
 
 
 Q4_BAD = [dict(x=None), dict(w=None), dict(s=None), dict(y=None), dict(ldx=95), dict(ldw=32), dict(ldw=56), dict(ldy=31),
@@ -71,6 +71,19 @@ Q4_BAD = [dict(x=None), dict(w=None), dict(s=None), dict(y=None), dict(ldx=95), 
 def test_linear_q4_refuses(rk_lib, bad):
     assert _q4(rk_lib, **bad) == REFUSED
     assert b"rk_linear_q4" in rk_lib.rk_last_error()
+
+
+def test_linear_q4_workspace(rk_lib):
+    """The size is pure arithmetic: it grows with rows and k, and a smaller, missing or misaligned one is refused."""
+    size = rk_lib.rk_linear_q4_workspace_size
+    assert size(0, 32, 96, 32, F32) == 0
+    for bad in [(-1, 32, 96, 32, F32), (1, 0, 96, 32, F32), (1, 32, 0, 32, F32), (1, 32, 96, 48, F32), (1, 32, 96, 32, 5)]:
+        assert size(*bad) == 0
+    assert 0 < size(1, 32, 96, 32, F16) < size(1, 32, 96, 32, F32) < size(1, 32, 4096, 32, F32) < size(33, 32, 4096, 32, F32)
+    need = size(4, 32, 96, 32, F32)
+    assert need % 256 == 0
+    for bad in (dict(ws=None), dict(ws=P + 128), dict(size=need - 1)):
+        assert _q4(rk_lib, **bad) == -2
 
 
 @pytest.mark.parametrize("bad", [dict(w=None), dict(q=None), dict(s=None), dict(ldw=95), dict(ldq=32), dict(ldq=56),
