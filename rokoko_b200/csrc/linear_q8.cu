@@ -303,7 +303,7 @@ struct Operands {
 
 // Tile sizes: the least estimated time over R in steps of 8 and C in steps of 16.  Measured on B200, in clocks of a
 // block of K: its four MMAs take 4 max(C / 2, 66), its bytes come at about 72 a clock and SM from L2 when all SMs
-// pull, and its two copies take their threads 205 (140 with two blocks a stage).  An SM's tiles take their blocks of
+// pull.  An SM's tiles take their blocks of
 // K, or their epilogues where those are longer; the last epilogue stands alone.
 void plan_tiles(const Q8Args& a, int sms, Q8Plan& p) {
     const int kb = (a.k + Q8_KB - 1) / Q8_KB;
