@@ -323,6 +323,25 @@ def test_linear_q4_keeps_32_bit_inputs(lin):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [3, 40])
+def test_linear_q4_uneven_magnitudes(lin, dtype, rows):
+    """Rows of zeros, of the type's smallest numbers, of magnitudes around and beyond 2^30 apart, each beside ordinary
+    rows: the ones that the 8-bit parts hold and the ones that they do not."""
+    g = gen(17)
+    k = 700
+    x = randn(g, rows, k, dtype=dtype)
+    x[0] = 0
+    x[1, ::3] *= 2.0 ** -14
+    x[2, 5] = 2.0 ** 15 if dtype == F16 else 2.0 ** 60
+    x[2, 6:] *= 2.0 ** -10
+    x[rows - 1] = (x[rows - 1] * TINY[dtype] * 8).to(dtype)
+    w, s, z = q4_case(g, 60, k, 64, F32, True)
+    ref, err = q4_ref(x, w, s, z, 64, None, None)
+    close(lin.linear_q4(x, w, s, 64, zeros=z), ref, err + TINY[F32] * k, dtype)
+    lin.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_linear_q4_strides_pads_and_in_place(lin, dtype):
     g, rows, n, k = gen(13), 5, 45, 250
     x = randn(g, rows, k, dtype=dtype)
@@ -422,6 +441,7 @@ def test_norm_then_linears(lin):
     ref, err = q4_ref(m, w2q, s2, z2, 64, None, h1)
     close(out, ref, err, F32)
     # and near the unquantised layer: 8-bit operands are off by 2^-4 / sqrt(3) a value at most, 4-bit ones by less
+    lin.check()
     full = norm_ref(y_ref @ w1.double().t() + b1.double(), n2)[1] @ w2.double().t() + h_ref
     assert float((out.double() - full).norm() / full.norm()) < 0.1
 
