@@ -108,6 +108,8 @@ __global__ void __launch_bounds__(256) q4_parts_kernel(const Q4Args a, const Q4P
     const int pass = p.pass0 + blockIdx.y / Q4_ROWS, m = blockIdx.y % Q4_ROWS;
     const long long row = (long long)pass * Q4_ROWS + m;
     if (row >= a.rows) return;
+    // The product may start when every block of this launch has: it fetches weights until it needs the parts.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     uint8_t* ws = a.ws + (size_t)pass * p.pass_bytes;
     auto load8 = [&](long long c, float (&v)[8]) {
@@ -254,7 +256,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
     const uint32_t tmem = tmem_sh;
     float* red = reinterpret_cast<float*>(ring);  // [sets][rows][128], once the ring is done with
 
-    if (warp == 0) {  // x: one copy a step
+    if (warp == 0) {  // x: one copy a step, once the first launch is done
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         int i = 0, s = 0;
         uint32_t parity = 1;
         for (; i < p.steps; i++) {
@@ -467,6 +470,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
         tmem_dealloc(tmem, p.tmem_cols);
     }
     if (lost) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the first launch's rows, here read plainly
     const Q4Row* info = reinterpret_cast<const Q4Row*>(ws + (size_t)p.steps * p.x_stage);
     for (int m = 0; m < rows; m++) {
         const Q4Row r = info[m];
@@ -579,7 +583,18 @@ cudaError_t launch_mb(const Q4Args& a, cudaStream_t st) {
         const int rows = n > 1 ? n * Q4_ROWS : (a.rows - p.pass0 * Q4_ROWS < Q4_ROWS ? a.rows - p.pass0 * Q4_ROWS : Q4_ROWS);
         const int slices = (p.h * p.steps + 15) / 16;  // 16 blocks of K a block: two a warp
         q4_parts_kernel<T><<<dim3(slices, rows), 256, 0, st>>>(a, p);
-        kernel<<<dim3((unsigned)grid, n), Q4_THREADS, smem, st>>>(a, p);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid, n);
+        cfg.blockDim = dim3(Q4_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, kernel, a, p);
+        if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
 }

@@ -203,7 +203,10 @@ constexpr int MAX_STAGES = 4;
 // residual on their way into a ring of `stages` slots of shared memory (a bulk
 // copy each) while one row is worked on in registers.  The copies move the
 // granules around a row, so rows may start anywhere (VEC = 1 then reads single
-// elements from shared memory).
+// elements from shared memory).  Bound by memory: 16384 x 8192 bf16 with a
+// residual, 8-bit output, 168 us = 5.6 TB/s, 87 % of a plain copy's rate, against
+// 178 to 309 us a row a block; rows off the 16-byte grid 342 us, where single
+// elements' instructions are the cost.
 template <typename T, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     norm_stream_kernel(const NormArgs a, int stages, uint32_t slot_bytes) {
@@ -349,6 +352,7 @@ cudaError_t launch_vec(const NormArgs& a, cudaStream_t st) {
     const int vectors = (a.cols + VEC - 1) / VEC;
     constexpr int E8 = VEC >= 8 ? 1 : 8 / VEC, E16 = 16 / VEC, E32 = 32 / VEC;  // vectors that make so many elements
     if (a.cols <= 1024) {
+        // many short rows: 8 lanes a row keep the reductions few (31000 x 256 f32, 8-bit output: 22.5 us, a warp a row 24.6)
         const bool many = a.rows >= 8 * sm_count();
         if (many && vectors <= 8 * E16) launch_group<T, VEC, E16, 8>(a, st);
         else if (many && vectors <= 16 * E16) launch_group<T, VEC, E16, 16>(a, st);

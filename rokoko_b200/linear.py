@@ -18,6 +18,8 @@ recorded.  There is no other path than librokoko_b200.so.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import lib
@@ -210,6 +212,11 @@ def linear_q8(x, x_scale, w, w_scale, bias=None, residual=None, dtype=torch.floa
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _q4_workspace(rows: int, n: int, k: int, group: int, dt: int) -> int:
+    return lib.load().rk_linear_q4_workspace_size(rows, n, k, group, dt)
+
+
 def _check_group(group) -> None:
     if not (group in (32, 64) or (group >= 128 and group % 128 == 0)):
         raise ValueError(f"group: 32, 64 or a multiple of 128 expected, got {group}")
@@ -266,7 +273,7 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
             raise ValueError("zeros: a contiguous tensor is expected")
         zp = zeros.data_ptr()
     out, tail = _finish_args(x, rows, n, dtype, dev, bias, residual, out)
-    size = lib.load().rk_linear_q4_workspace_size(rows, n, k, group, dt)
+    size = _q4_workspace(rows, n, k, group, dt)
     ws = x.new_empty((size,), dtype=torch.uint8)  # torch's blocks start on 512-byte boundaries
     _call("rk_linear_q4", dev, x.data_ptr(), ldx, pw, ldw, scales.data_ptr(), zp, *tail, ws.data_ptr(), size, rows, n, k,
           group, dt, st)
