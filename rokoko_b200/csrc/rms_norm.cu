@@ -205,8 +205,8 @@ constexpr int MAX_STAGES = 4;
 // granules around a row, so rows may start anywhere (VEC = 1 then reads single
 // elements from shared memory).  Bound by memory: 16384 x 8192 bf16 with a
 // residual, 8-bit output, 168 us = 5.6 TB/s, 87 % of a plain copy's rate, against
-// 178 to 309 us a row a block; rows off the 16-byte grid 342 us, where single
-// elements' instructions are the cost.
+// 178 to 309 us a row a block.  With VEC = 1 single elements' instructions are the
+// cost (8191 columns: 336 us); norm_shifted_kernel takes most such rows.
 template <typename T, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     norm_stream_kernel(const NormArgs a, int stages, uint32_t slot_bytes) {
@@ -285,6 +285,155 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
             }
 }
 
+// norm_stream_kernel for rows off the 16-byte grid.  Elements are worked on where
+// they lie, in vectors that are aligned in x, the residual, the sum and y, all of
+// which begin at the same place within 16 bytes.  A block's rows are a multiple of
+// 8 rows apart, so each begins `skip` elements into its first vector.  The 8-bit
+// rows lie on a grid of their own: a lane puts the rest of its vector's codes and
+// the start of its right neighbour's together, and only the seams between warps go
+// out by single bytes.  Against single elements, with a residual and 8-bit output:
+// 16384 x 8185 bf16 217 us (4.3 TB/s) for 336, 8000 x 8001 f32 136 for 208, 16384 x
+// 4001 f16 113 for 178; 16384 x 8191 bf16, one block an SM, 295 for 336.
+template <typename T, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+    norm_shifted_kernel(const NormArgs a, int stages, uint32_t slot_bytes) {
+    constexpr int VEC = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t slots[];
+    __shared__ __align__(8) uint64_t bar[MAX_STAGES];
+    __shared__ float2 red[2][32];
+    using P = Pack<T, VEC>;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int first = tid / 32 * (32 * NV) + lane;  // a warp's vectors lie together
+    const long long step = gridDim.x;
+    const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T), stage_bytes = slot_bytes * (a.res ? 2 : 1);
+    const int skip = (int)((a.xoff + (long long)blockIdx.x * a.ldx * (long long)sizeof(T)) & 15) / (int)sizeof(T);
+    if (tid == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(&bar[s], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    auto load = [&](long long row, int s) {  // one thread
+        const char *px, *pr;
+        const uint32_t nx = granules(static_cast<const T*>(a.x) + row * a.ldx, row_bytes, &px);
+        uint32_t nr = 0;
+        if (a.res) nr = granules(static_cast<const T*>(a.res) + row * a.ldr, row_bytes, &pr);
+        mbar_arrive_expect_tx(&bar[s], nx + nr);
+        bulk_load(slots + (size_t)s * stage_bytes, px, nx, &bar[s]);
+        if (a.res) bulk_load(slots + (size_t)s * stage_bytes + slot_bytes, pr, nr, &bar[s]);
+    };
+    long long row = blockIdx.x;
+    if (tid == 0)
+        for (int s = 0; s < stages; s++)
+            if (row + s * step < a.rows) load(row + s * step, s);
+    P pw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            const int c = (first + i * 32) * VEC - skip + j;
+            pw[i].v[j] = a.w && c >= 0 && c < a.cols ? static_cast<const T*>(a.w)[c] : from_f32<T>(0.f);
+        }
+    int s = 0, flip = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (; row < a.rows; row += step) {
+        ok = mbar_wait(&bar[s], parity, &norm_err, RK_DEV_TIMEOUT_FULL);
+        const uint8_t* slot = slots + (size_t)s * stage_bytes;
+        float hw[NV][VEC];
+        RowPart<T, VEC> p;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int at = first + i * 32, c = at * VEC - skip;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) hw[i][j] = 0.f;
+            if (c < a.cols) {
+                P px = *reinterpret_cast<const P*>(slot + at * 16), pr;
+                if (a.res) pr = *reinterpret_cast<const P*>(slot + slot_bytes + at * 16);
+                T* sum = a.sum && ok ? static_cast<T*>(a.sum) + row * a.lds + c : nullptr;
+                if (c >= 0 && c + VEC <= a.cols) {
+                    p.add(px, pr, pw[i], a.res, a.w, sum, hw[i]);
+                } else {  // the row's ends: what does not belong to it counts as zeros
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        if (c + j < 0 || c + j >= a.cols) { px.v[j] = from_f32<T>(0.f); pr.v[j] = from_f32<T>(0.f); }
+                    p.add(px, pr, pw[i], a.res, a.w, nullptr, hw[i]);
+                    if (sum) {
+#pragma unroll
+                        for (int j = 0; j < VEC; j++)
+                            if (c + j >= 0 && c + j < a.cols)
+                                sum[j] = from_f32<T>(to_f32(px.v[j]) + (a.res ? to_f32(pr.v[j]) : 0.f));
+                    }
+                }
+            }
+        }
+        ok = p.reduce_block(red[flip], ok);
+        flip ^= 1;
+        if (!ok) break;  // the same for the whole block
+        if (tid == 0 && row + stages * step < a.rows) load(row + stages * step, s);
+        if (++s == stages) { s = 0; parity ^= 1; }
+        const RowFactors f(a, p.ss, p.top);
+        if (a.q && tid == 0) a.scale[row] = f.scale;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (first + i * 32) * VEC - skip;
+            if (a.y && c < a.cols) {
+                P o;
+                T* y = static_cast<T*>(a.y) + row * a.ldy + c;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) o.v[j] = from_f32<T>(hw[i][j] * f.y);
+                if (c >= 0 && c + VEC <= a.cols) {
+                    *reinterpret_cast<P*>(y) = o;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        if (c + j >= 0 && c + j < a.cols) y[j] = o.v[j];
+                }
+            }
+        }
+        if (!a.q) continue;
+        uint64_t own[NV];  // every lane's: its neighbour may need them
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            Codes<8> k = {};
+            store_codes<VEC>(k.v, hw[i], f.q);
+            own[i] = *reinterpret_cast<const uint64_t*>(&k);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int to = (first + i * 32) * VEC, left = a.cols - to;
+            uint64_t next = __shfl_down_sync(0xffffffffu, own[i], 1);
+            if (i + 1 < NV) {
+                const uint64_t after = __shfl_sync(0xffffffffu, own[i + 1 < NV ? i + 1 : i], 0);
+                if (lane == 31) next = after;
+            }
+            const bool tail = i == NV - 1 && lane == 31, head = i == 0 && lane == 0 && tid > 0;
+            uint8_t* q = a.q + row * a.ldq + to;
+            uint64_t all = own[i] >> (8 * skip);
+            if (skip) all |= next << (8 * (VEC - skip));
+            if (!tail && left >= VEC) {
+                if constexpr (VEC == 8) *reinterpret_cast<uint64_t*>(q) = all;
+                else *reinterpret_cast<uint32_t*>(q) = (uint32_t)all;
+            } else if (!tail && left > 0) {
+                for (int j = 0; j < left; j++) q[j] = (uint8_t)(all >> (8 * j));
+            }
+            if (i == 0 || i == NV - 1) {  // the seam between two warps: each stores its own
+                const int count = head ? min(skip, left + skip) : tail ? min(left, VEC - skip) : 0;
+                uint8_t* at = head ? q - skip : q;
+                const uint64_t codes = head ? own[i] : all;
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if (j < count) at[j] = (uint8_t)(codes >> (8 * j));
+            }
+        }
+    }
+    if (!ok && tid == 0)  // a wait gave up: no copy may outlive the block
+        for (int k = 0; k < stages; k++)
+            if (row + k * step < a.rows) {
+                const int q = s + k < stages ? s + k : s + k - stages;
+                mbar_wait(&bar[q], s + k < stages ? parity : parity ^ 1, &norm_err, RK_DEV_TIMEOUT_DRAIN);
+            }
+}
+
 // Rows that do not fit one block's registers: read twice, the second time from L2.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_long_rows_kernel(const NormArgs a) {
@@ -324,9 +473,12 @@ void launch_block(const NormArgs& a, int vectors, cudaStream_t st) {
     norm_rows_kernel<T, VEC, NV, 0><<<a.rows, threads, 0, st>>>(a);
 }
 
-template <typename T, int VEC, int NV, int THREADS>
+// SHIFTED: rows off the 16-byte grid in vectors (VEC elements), as norm_shifted_kernel takes them
+template <typename T, int VEC, int NV, int THREADS, bool SHIFTED = false>
 cudaError_t launch_stream(const NormArgs& a, int vectors, cudaStream_t st) {
-    auto kernel = norm_stream_kernel<T, VEC, NV, THREADS>;
+    void (*kernel)(NormArgs, int, uint32_t);
+    if constexpr (SHIFTED) kernel = norm_shifted_kernel<T, NV, THREADS>;
+    else kernel = norm_stream_kernel<T, VEC, NV, THREADS>;
     static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -342,7 +494,8 @@ cudaError_t launch_stream(const NormArgs& a, int vectors, cudaStream_t st) {
     while (ctas > 1 && RING_BYTES / ctas < 2 * stage) ctas--;
     int stages = RING_BYTES / ctas / stage;
     stages = stages > MAX_STAGES ? MAX_STAGES : stages;
-    const long long grid = (long long)ctas * sm_count();
+    long long grid = (long long)ctas * sm_count();
+    if (SHIFTED) grid = grid / 8 * 8;  // 8 rows of any length are whole vectors
     kernel<<<(int)(a.rows < grid ? a.rows : grid), threads, (size_t)stages * stage, st>>>(a, stages, (uint32_t)slot);
     return cudaSuccess;
 }
@@ -376,9 +529,18 @@ cudaError_t launch(const NormArgs& a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(T);
     const bool one = a.rows == 1;
     auto fits = [&](const void* p, long long ld, size_t e) { return aligned(p, VEC * e) && (one || ld % VEC == 0); };
+    // rows that begin at the same place within 16 bytes, wherever that is
+    auto with_x = [&](const void* p, long long ld) {
+        return !p || (((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(a.x)) & 15) == 0 && (ld - a.ldx) % VEC == 0);
+    };
+    const int most = (a.cols + 2 * VEC - 2) / VEC;  // vectors that a row may touch
     const bool vec = a.cols % VEC == 0 && fits(a.x, a.ldx, sizeof(T)) && fits(a.w, 0, sizeof(T)) &&
                      fits(a.res, a.ldr, sizeof(T)) && fits(a.sum, a.lds, sizeof(T)) && fits(a.y, a.ldy, sizeof(T)) &&
                      fits(a.q, a.ldq, 1);
+    if (!vec && a.cols > 1024 && most <= 1024 * (16 / VEC) && a.rows > 4 * sm_count() && with_x(a.res, a.ldr) &&
+        with_x(a.sum, a.lds) && with_x(a.y, a.ldy) && (!a.q || (aligned(a.q, VEC) && a.ldq % VEC == 0)))
+        return most <= 512 * (16 / VEC) ? launch_stream<T, VEC, 16 / VEC, 512, true>(a, most, st)
+                                        : launch_stream<T, VEC, 16 / VEC, 1024, true>(a, most, st);
     if (a.cols <= MAX_COLS) return vec ? launch_vec<T, VEC>(a, st) : launch_vec<T, 1>(a, st);
     norm_long_rows_kernel<T><<<a.rows, 1024, 0, st>>>(a);
     return cudaSuccess;

@@ -140,6 +140,43 @@ def test_norm_strides_and_in_place(lin, dtype, cols):
         assert torch.equal(br[:, keep], wide_r[:, keep])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("cols", [1025, 1536, 2037, 4099, 8185, 8191, 8192, 12001])
+@pytest.mark.parametrize("off,gap,apart", [(0, 8, 0), (0, 0, 0), (1, 13, 0), (3, 16, 0), (4, 9, 0), (7, 7, 0), (2, 11, 8),
+                                           (5, 11, 1)])
+def test_norm_many_rows(lin, dtype, cols, off, gap, apart):
+    """Rows enough for every block to work on several, from any place within 16 bytes, the residual's rows `apart`
+    elements from there; NaN before and behind every row must not get in."""
+    rows, ld = 1601, cols + gap
+    g = gen(off * 11 + cols)
+    flat = randn(g, 2, rows * ld + 32, dtype=dtype)
+    x = flat[0].as_strided((rows, cols), (ld, 1), off)
+    r = flat[1].as_strided((rows, cols), (ld, 1), flat.stride(0) + off + apart)
+    xs, rs = x.clone(), r.clone()
+    flat.fill_(float("nan"))
+    x.copy_(xs)
+    r.copy_(rs)
+    w = randn(g, cols, dtype=dtype)
+    h_ref, y_ref = norm_ref(xs, w, rs)
+    q, s, h = lin.rms_norm_q8(x, w, residual=r, eps=EPS)
+    check_q8(q, s, y_ref)
+    close(h, h_ref, h_ref.abs() * U, dtype)
+    q1, s1 = lin.rms_norm_q8(x, w, eps=EPS)
+    check_q8(q1, s1, norm_ref(xs, w)[1])
+    q2, s2 = lin.quantize_q8(x)
+    check_q8(q2, s2, xs.double(), rel=2 * U)
+    y, h = lin.rms_norm(x, w, residual=r, eps=EPS)
+    close(y, y_ref, y_ref.abs() * 64 * U, dtype)
+    close(h, h_ref, h_ref.abs() * U, dtype)
+    y1, h1 = lin.rms_norm(x, w, residual=r, eps=EPS, out=x, sum_out=r)
+    close(y1, y_ref, y_ref.abs() * 64 * U, dtype)
+    assert torch.equal(h1, h)
+    left = torch.ones(flat.shape, dtype=torch.bool, device="cuda")
+    left[0].as_strided((rows, cols), (ld, 1), off).fill_(False)
+    left[1].as_strided((rows, cols), (ld, 1), left.stride(0) + off + apart).fill_(False)
+    assert torch.isnan(flat[left]).all() and not torch.isnan(flat[~left]).any()
+
+
 @pytest.mark.parametrize("cols", [64, 513, 4096, 40000])
 def test_norm_rows_of_zeros_nan_and_infinity(lin, cols):
     """A row's zeros, NaN or infinity stay in that row."""
