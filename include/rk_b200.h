@@ -135,8 +135,10 @@ RK_API rk_status rk_conv1d_static_check(void* stream);
  * Activations, norm weights and residuals are RK_DTYPE_* elements; every sum,
  * norm and scale is held in 32 bits and rounded once, to nearest, when a result
  * is stored.  Row pitches (ld*) count elements and are at least the row's
- * length; a single row's pitch is not looked at.  rows = 0 does nothing.  An
- * unsupported argument gives RK_ERR_CANNOT_IMPLEMENT and enqueues nothing.
+ * length; a single row's pitch is not looked at.  Rows and columns go up to 2^30.
+ * Outputs overlap no input but where an entry point says so.  rows = 0 does
+ * nothing.  An unsupported argument gives RK_ERR_CANNOT_IMPLEMENT and enqueues
+ * nothing.
  *
  * 8-bit rows ("q8"): e4m3 codes with one float scale a row, value = scale x
  * code.  scale = max(max|y|, 1e-30) / 448, so a row of zeros has zero codes.  A

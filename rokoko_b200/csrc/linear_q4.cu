@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(256)
     const int g = (int)(unit - row * groups);
     if (row >= n) return;
     const T* src = w + row * ldw;
-    const int k0 = g * group, k1 = k0 + group < k ? k0 + group : k;
+    const int k0 = g * group, k1 = k - k0 > group ? k0 + group : k;
     float lo = 0.f, hi = 0.f;
     for (int c = k0 + lane; c < k1; c += 32) {
         const float v = to_f32(src[c]);
@@ -693,7 +693,7 @@ void* q4_err_word() {
 using namespace rk;
 
 extern "C" size_t rk_linear_q4_workspace_size(int rows, int n, int k, int group, int dtype) {
-    if (rows < 0 || n < 1 || k < 1 || !group_ok(group) || !dtype_ok(dtype)) return 0;
+    if (!size_ok(rows, 0) || !size_ok(n, 1) || !size_ok(k, 1) || !group_ok(group) || !dtype_ok(dtype)) return 0;
     return rows ? workspace_bytes(rows, k, group, dtype) : 0;
 }
 
@@ -702,7 +702,8 @@ extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, l
                                   void* y, long long ldy, void* workspace, size_t workspace_size, int rows, int n,
                                   int k, int group, int dtype, int scale_dtype, void* stream) {
     const char* who = "rk_linear_q4: unsupported arguments";
-    if (!dtype_ok(dtype) || !dtype_ok(scale_dtype) || rows < 0 || n < 1 || k < 1) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
+    if (!dtype_ok(dtype) || !dtype_ok(scale_dtype) || !size_ok(rows, 0) || !size_ok(n, 1) || !size_ok(k, 1))
+        return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     if (!group_ok(group))
         return fail(RK_ERR_CANNOT_IMPLEMENT, "rk_linear_q4: groups are of 32, 64 or a multiple of 128 columns");
     if (rows == 0) return RK_OK;
@@ -732,7 +733,8 @@ extern "C" rk_status rk_quantize_q4(const void* w, long long ldw, void* q, long 
                                     uint8_t* zeros, int n, int k, int group, int dtype, int scale_dtype,
                                     void* stream) {
     const char* who = "rk_quantize_q4: unsupported arguments";
-    if (!dtype_ok(dtype) || !dtype_ok(scale_dtype) || n < 0 || k < 1) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
+    if (!dtype_ok(dtype) || !dtype_ok(scale_dtype) || !size_ok(n, 0) || !size_ok(k, 1))
+        return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     if (!group_ok(group))
         return fail(RK_ERR_CANNOT_IMPLEMENT, "rk_quantize_q4: groups are of 32, 64 or a multiple of 128 columns");
     if (n == 0) return RK_OK;

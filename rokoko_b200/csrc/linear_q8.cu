@@ -371,7 +371,8 @@ extern "C" rk_status rk_linear_q8(const void* x, long long ldx, const float* x_s
                                   const float* w_scale, const float* bias, const void* residual, long long ldr,
                                   void* y, long long ldy, int rows, int n, int k, int dtype, void* stream) {
     const char* who = "rk_linear_q8: unsupported arguments";
-    if (!dtype_ok(dtype) || rows < 0 || n < 1 || k < 1) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
+    if (!dtype_ok(dtype) || !size_ok(rows, 0) || !size_ok(n, 1) || !size_ok(k, 1))
+        return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     if (rows == 0) return RK_OK;
     const size_t e = dtype_bytes(dtype);
     if (!x || !x_scale || !w || !w_scale || !y || !pitch_ok(ldx, rows, k) || !pitch_ok(ldw, n, k) ||

@@ -547,7 +547,7 @@ cudaError_t launch(const NormArgs& a, cudaStream_t st) {
 }
 
 rk_status norm_rows(const NormArgs& a, bool norm, int dtype, void* stream, const char* who) {
-    if (!dtype_ok(dtype) || a.rows < 0 || a.cols < 1) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
+    if (!dtype_ok(dtype) || !size_ok(a.rows, 0) || !size_ok(a.cols, 1)) return fail(RK_ERR_CANNOT_IMPLEMENT, who);
     if (a.rows == 0) return RK_OK;
     if (!a.x || (norm && !a.w) || (!a.y && !(a.q && a.scale)) || !pitch_ok(a.ldx, a.rows, a.cols) ||
         (a.res && !pitch_ok(a.ldr, a.rows, a.cols)) || (a.sum && !pitch_ok(a.lds, a.rows, a.cols)) ||

@@ -96,6 +96,23 @@ def test_quantize_q4_refuses(rk_lib, bad):
     assert b"rk_quantize_q4" in rk_lib.rk_last_error()
 
 
+BIG = (1 << 30) + 1
+
+
+def test_more_than_2_30_rows_or_columns_are_refused(rk_lib):
+    """32-bit indices would step past the end by a block's width."""
+    for name in ("rk_rms_norm", "rk_rms_norm_q8", "rk_quantize_q8"):
+        assert _norm(rk_lib, name, cols=BIG, ldx=2 * BIG, ldy=2 * BIG) == REFUSED
+        assert _norm(rk_lib, name, rows=BIG) == REFUSED
+    for bad in (dict(rows=BIG), dict(n=BIG, ldy=2 * BIG), dict(k=BIG, ldx=1 << 32, ldw=1 << 32)):
+        assert _q8(rk_lib, **bad) == REFUSED
+        assert _q4(rk_lib, **bad) == REFUSED
+        a = dict(rows=1, n=32, k=96) | {k: v for k, v in bad.items() if k in ("rows", "n", "k")}
+        assert rk_lib.rk_linear_q4_workspace_size(a["rows"], a["n"], a["k"], 32, F32) == 0
+    assert rk_lib.rk_quantize_q4(P, 1 << 32, P, 1 << 32, P, None, 1, BIG, 1 << 30, F32, F32, None) == REFUSED
+    assert rk_lib.rk_quantize_q4(P, 96, P, 48, P, None, BIG, 96, 128, F32, F32, None) == REFUSED
+
+
 def test_zero_rows_are_no_work(rk_lib):
     for name in ("rk_rms_norm", "rk_rms_norm_q8", "rk_quantize_q8"):
         assert _norm(rk_lib, name, rows=0, x=None, y=None) == 0
