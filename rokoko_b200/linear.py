@@ -11,7 +11,9 @@
 Tensors are 2-D CUDA tensors [rows, columns] whose columns are adjacent (any
 row stride), in float32, float16 or bfloat16; what a call reads and writes
 stands at the entry points of include/rk_b200.h.  Results are new tensors on
-the current stream of the inputs' device.  Arguments that do not fit raise
+the current stream of the inputs' device, or the ones that `out` and `sum_out`
+name; these may be an input itself where a function says so and otherwise share
+no memory with x, the residual or each other.  Arguments that do not fit raise
 ValueError before anything is enqueued.  The operators are for serving and have
 no gradients: an input that requires one is refused while gradients are
 recorded.  There is no other path than librokoko_b200.so.
@@ -73,6 +75,27 @@ def _vector(t, name: str, dtype, dev: int, n: int) -> int:
     return t.data_ptr()
 
 
+def _apart(out, other, what: str, itself: bool = False) -> None:
+    """Refuses an output that shares memory with `other`, a tensor of the same rows; `itself`: the very same rows may.
+    Columns of one buffer beside each other are apart."""
+    if out is None or other is None or not out.numel():
+        return
+    a, b = out.data_ptr(), other.data_ptr()
+    lda, ldb = out.stride(0) * out.element_size(), other.stride(0) * other.element_size()
+    wa, wb = out.shape[1] * out.element_size(), other.shape[1] * other.element_size()
+    one = out.shape[0] == 1
+    if itself and a == b and (one or lda == ldb):
+        return
+    far = 0 if one else out.shape[0] - 1
+    if a + far * lda + wa <= b or b + far * ldb + wb <= a:
+        return
+    if not one and lda == ldb:
+        at = (b - a) % lda
+        if at >= wa and at + wb <= lda:
+            return
+    raise ValueError(f"{what} overlap")
+
+
 def _activation(x, name: str = "x"):
     """(dtype code, device, rows, columns) of the tensor that sets them for a call."""
     if not isinstance(x, torch.Tensor):
@@ -122,6 +145,8 @@ def _norm_args(x, weight, residual, sum_out):
     if sum_out is not None:
         lds = _rows(sum_out, "sum_out", x.dtype, dev, rows, cols)
         sp = sum_out.data_ptr()
+        _apart(sum_out, x, "sum_out and x", itself=True)
+        _apart(sum_out, residual, "sum_out and residual", itself=True)
     elif residual is not None:
         sum_out, lds = x.new_empty((rows, cols)), cols
         sp = sum_out.data_ptr()
@@ -140,6 +165,9 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
         ldy = _rows(out, "out", x.dtype, dev, rows, cols)
         if not (h is None or h.data_ptr() != out.data_ptr() or rows == 0):
             raise ValueError("out and sum_out are the same memory")
+        _apart(out, sum_out, "out and sum_out")
+        _apart(out, x, "out and x", itself=True)
+        _apart(out, residual, "out and residual", itself=True)
     _call("rk_rms_norm", dev, *args, out.data_ptr(), ldy, rows, cols, eps, dt)
     return out if h is None else (out, h)
 
@@ -164,16 +192,18 @@ def quantize_q8(x):
     return q, scale
 
 
-def _finish_args(like, rows: int, n: int, dtype, dev: int, bias, residual, out):
+def _finish_args(x, rows: int, n: int, dtype, dev: int, bias, residual, out):
     bp = _vector(bias, "bias", torch.float32, dev, n) if bias is not None else None
     rp, ldr = None, 0
     if residual is not None:
         ldr = _rows(residual, "residual", dtype, dev, rows, n)
         rp = residual.data_ptr()
     if out is None:
-        out, ldy = like.new_empty((rows, n), dtype=dtype), n
+        out, ldy = x.new_empty((rows, n), dtype=dtype), n
     else:
         ldy = _rows(out, "out", dtype, dev, rows, n)
+        _apart(out, residual, "out and residual", itself=True)
+        _apart(out, x, "out and x")
     return out, (bp, rp, ldr, out.data_ptr(), ldy)
 
 

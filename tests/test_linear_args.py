@@ -141,6 +141,29 @@ def test_python_front_end_refuses_host_tensors():
         linear.rms_norm(x.double(), w)
 
 
+def test_overlapping_rows():
+    """Which rows the front end takes to share memory, against the sets of their elements."""
+    torch = pytest.importorskip("torch")
+    from rokoko_b200.linear import _apart
+    buf = torch.zeros(400)
+    seen = set()
+    for rows, cols, la, lb, at in [(r, c, a, b, o) for r in (1, 3) for c in (4, 7) for a in (16, 20) for b in (16, 20)
+                                   for o in (0, 1, 4, 7, 9, 12, 13, 16, 33, 60, 80)]:
+        a, b = buf.as_strided((rows, cols), (la, 1), 100), buf.as_strided((rows, cols), (lb, 1), 100 + at)
+        for x, y in ((a, b), (b, a)):
+            where = [{(t.data_ptr() // 4 + i * t.stride(0) + j) for i in range(rows) for j in range(cols)} for t in (x, y)]
+            try:
+                _apart(x, y, "x and y")
+                free = True
+            except ValueError:
+                free = False
+            assert not (free and where[0] & where[1])                       # never let through
+            assert free or where[0] & where[1] or (rows > 1 and la != lb)   # refused in vain for unlike pitches alone
+            seen.add(free)
+    assert seen == {True, False}
+    _apart(buf.view(20, 20)[:, :4], buf.view(20, 20)[:, :4], "x and y", itself=True)
+
+
 def test_header_constants_match():
     from rokoko_b200 import lib
     assert (lib.RK_DTYPE_F32, lib.RK_DTYPE_F16, lib.RK_DTYPE_BF16) == (F32, F16, BF16)

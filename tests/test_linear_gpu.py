@@ -577,6 +577,40 @@ def test_refusals(lin):
         lin.quantize_q4(x, 100)
 
 
+def test_outputs_that_overlap_inputs_are_refused(lin):
+    """Rows are worked on side by side, so an output may share memory with an input only row on row."""
+    g = gen(9)
+    buf = randn(g, 9, 200)
+    w, x, side = randn(g, 64), buf[:8, :64], buf[:8, 64:128]
+    with pytest.raises(ValueError, match="out and x overlap"):
+        lin.rms_norm(x, w, out=buf[1:, :64])
+    with pytest.raises(ValueError, match="out and x overlap"):
+        lin.rms_norm(x, w, out=buf[:8, 32:96])
+    with pytest.raises(ValueError, match="out and residual overlap"):
+        lin.rms_norm(x.clone(), w, residual=x, out=buf[:8, 1:65])
+    with pytest.raises(ValueError, match="sum_out and x overlap"):
+        lin.rms_norm_q8(x, w, sum_out=buf[1:, :64])
+    with pytest.raises(ValueError, match="sum_out and residual overlap"):
+        lin.rms_norm_q8(x.clone(), w, residual=x, sum_out=buf[:8, 1:65])
+    with pytest.raises(ValueError, match="out and sum_out overlap"):
+        lin.rms_norm(x.clone(), w, out=x, sum_out=buf[:8, 32:96])
+    p4, s4, _ = lin.quantize_q4(randn(g, 64, 64), 32)
+    with pytest.raises(ValueError, match="out and x overlap"):
+        lin.linear_q4(x, p4, s4, 32, out=x)
+    with pytest.raises(ValueError, match="out and residual overlap"):
+        lin.linear_q4(x.clone(), p4, s4, 32, residual=x, out=buf[1:, :64])
+    # beside each other, the columns between them of others, they are apart
+    ref = lin.rms_norm(x.clone(), w)
+    assert torch.equal(lin.rms_norm(x, w, out=side), ref)
+    ref = lin.linear_q4(x.clone(), p4, s4, 32)
+    assert torch.equal(lin.linear_q4(x, p4, s4, 32, out=side), ref)
+    assert torch.equal(lin.linear_q4(x, p4, s4, 32, out=buf[:8, 136:]), ref)
+    one = buf[8:]
+    assert torch.equal(lin.linear_q4(one[:, :64], p4, s4, 32, out=one[:, 64:128]), lin.linear_q4(one[:, :64], p4, s4, 32))
+    with pytest.raises(ValueError, match="out and x overlap"):
+        lin.linear_q4(one[:, :64], p4, s4, 32, out=one[:, 63:127])
+
+
 def test_zero_rows(lin):
     x, w = torch.zeros(0, 64, device="cuda"), torch.ones(64, device="cuda")
     assert lin.rms_norm(x, w).shape == (0, 64)
