@@ -32,22 +32,14 @@
 #include <atomic>
 
 #include "ptx.cuh"
+#include "q4_plan.h"
 #include "quant.cuh"
 #include "status.h"
 
 namespace rk {
 namespace {
 
-constexpr int Q4_ZERO = 8;     // the zero point of weights that have none of their own
-constexpr int Q4_KB = 128;     // columns of a block of K: a row of the 128-byte swizzle
-constexpr int Q4_ROWS = 32;    // most activation rows of a pass over the weights
-constexpr int Q4_M = 128;      // the MMA's weight rows
-constexpr int Q4_STAGES = 8;      // most stages
-constexpr int Q4_CODES = 8;       // warps that turn codes into operands
-constexpr int Q4_SUMS = 8;        // warps that add up accumulators
-constexpr int Q4_A_BYTES = Q4_M * Q4_KB;
-constexpr int Q4_THREADS = 32 * (2 + Q4_CODES + Q4_SUMS);  // and x copies, products
-constexpr int Q4_SMEM = 220 * 1024;
+constexpr int Q4_ZERO = 8;  // the zero point of weights that have none of their own
 
 template <typename T> struct Q4Type { static constexpr int PARTS = 3; };
 template <> struct Q4Type<float> { static constexpr int PARTS = 6; };
@@ -64,31 +56,6 @@ struct Q4Args {
     int rows, n, k, group, groups, s_dtype;
     bool x_vec;   // rows of x start on 16-byte boundaries
     uint8_t* ws;  // per pass: its steps' stages, then the rows' Q4Row
-};
-
-// What the parts of a row stand for.
-struct Q4Row {
-    float inv;  // 2^9 / the power of two that x was scaled by, as two factors
-    float inv2;
-    int odd;    // does not fit the parts
-    int pad;
-};
-
-// How a launch is divided, the same for all of its blocks.
-struct Q4Plan {
-    int h, pad;          // ranges of k below one another, weight rows set aside for each (128 / h)
-    int share;           // most weight rows of a block
-    int steps;           // blocks of K of a range
-    int sub;             // groups of a block of K: 4, 2, 1
-    int mq;              // activation rows of a pass, in fours
-    int nc;              // N columns of a range: parts x mq, in eights
-    uint32_t x_bytes, x_stage;  // of a step: the operand rows [h * nc][128] and after them the sums [h][sub][mq]
-    int stages;
-    uint32_t s_off, stage;      // shared memory: [128][sub] scales and zero points of a stage, a stage
-    uint32_t acc_cols, tmem_cols, idesc;
-    int accs;                   // accumulators: 4 where they fit, 2
-    size_t pass_bytes;   // workspace of a pass
-    int pass0;           // first pass of this launch
 };
 
 // ---------------------------------------------------------------- the parts of x
@@ -508,32 +475,10 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
 
 // ---------------------------------------------------------------- host
 
-int parts_of(int dtype) { return dtype == RK_DTYPE_F32 ? 6 : 3; }
-int sub_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
-
-// The widths that a pass has whatever the division: activation rows in fours, N columns of a range in eights.
-void pass_widths(int rows, int dtype, int& mq, int& nc) {
-    const int m = rows < Q4_ROWS ? rows : Q4_ROWS;
-    mq = (m + 3) / 4 * 4;
-    nc = (parts_of(dtype) * mq + 7) / 8 * 8;
-}
-
-// Workspace of a pass for a division into ranges of `steps` blocks of K.
-size_t pass_bytes(int rows, int group, int dtype, long long blocks) {
-    int mq, nc;
-    pass_widths(rows, dtype, mq, nc);
-    return (size_t)blocks * ((size_t)nc * 128 + (size_t)sub_of(group) * mq * 4) + Q4_ROWS * sizeof(Q4Row);
-}
-
-size_t workspace_bytes(int rows, int k, int group, int dtype) {
-    const long long passes = ((long long)rows + Q4_ROWS - 1) / Q4_ROWS, blocks = ((long long)k + Q4_KB - 1) / Q4_KB;
-    return (size_t)passes * ((pass_bytes(rows, group, dtype, blocks + 3) + 255) / 256 * 256);  // 4 even ranges of k
-}
-
 template <typename T, int MB, int SUB>
 cudaError_t launch_mb(const Q4Args& a, cudaStream_t st) {
     auto kernel = linear_q4_kernel<T, MB, SUB>;
-    Q4Plan p = {};
+    Q4Plan p;
     static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory is set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -543,40 +488,8 @@ cudaError_t launch_mb(const Q4Args& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    const int sms = sm_count(), blocks = (int)(((long long)a.k + Q4_KB - 1) / Q4_KB);
-    // an even share of the weight rows for each SM, in as many rounds as 128 rows a block make it
-    long long grid = sms;
-    while ((a.n + grid - 1) / grid > Q4_M) grid += sms;
-    if (grid > a.n) grid = a.n;
-    p.share = (int)((a.n + grid - 1) / grid);
-    p.h = p.share <= 32 ? 4 : p.share <= 64 ? 2 : 1;
-    while (p.h > blocks) p.h /= 2;
-    pass_widths(a.rows, sizeof(T) == 4 ? RK_DTYPE_F32 : RK_DTYPE_F16, p.mq, p.nc);
-    while (p.h > 1 && p.h * p.nc > 128) p.h /= 2;  // wide ones need no filling: their MMAs take as long as their N
-    p.pad = Q4_M / p.h;
-    p.steps = (blocks + p.h - 1) / p.h;
-    p.sub = SUB;
-    p.x_bytes = (uint32_t)(p.h * p.nc * 128);
-    p.x_stage = p.x_bytes + (uint32_t)(p.h * p.sub * p.mq * 4);
-    const int nn = (p.h * p.nc + 15) / 16 * 16;
-    p.idesc = umma_idesc_e4m3(Q4_M, nn) | 1u << 10;  // B in e5m2
-    p.acc_cols = (uint32_t)(nn + 31) / 32 * 32;
-    p.accs = 4 * p.acc_cols <= 512 ? 4 : 2;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < p.accs * p.acc_cols) p.tmem_cols *= 2;
-    p.pass_bytes = ((size_t)p.steps * p.x_stage + Q4_ROWS * sizeof(Q4Row) + 255) / 256 * 256;
-    // an MMA of N in sixteens may read eight rows past a stage's operand rows, which the scales' place makes up for
-    p.s_off = Q4_A_BYTES + (p.x_stage + 127) / 128 * 128;
-    p.stage = (p.s_off + Q4_M * p.sub * (uint32_t)sizeof(float2) + 1023) / 1024 * 1024;
-    p.stages = (Q4_SMEM - 1024) / (int)p.stage;
-    if (p.stages > Q4_STAGES) p.stages = Q4_STAGES;
-    // A warp of codes goes on Q4_CODES / 2 steps at a time.  With fewer stages it could be two rounds ahead of a stage's
-    // barrier, whose parity would let it through.
-    if (p.stages < Q4_CODES / 2) return cudaErrorInvalidConfiguration;
-    int smem = p.stages * (int)p.stage;
-    const int red = 2 * Q4_ROWS * Q4_M * 4;
-    if (smem < red) smem = red;
-    smem += 1024;
+    if (!q4_plan(a.rows, a.n, a.k, a.group, sizeof(T), sm_count(), p)) return cudaErrorInvalidConfiguration;
+    p.idesc = umma_idesc_e4m3(Q4_M, p.mma_n) | 1u << 10;  // B in e5m2
     const int passes = (int)(((long long)a.rows + Q4_ROWS - 1) / Q4_ROWS);
     for (p.pass0 = 0; p.pass0 < passes; p.pass0 += 2047) {  // rows and passes are the grids' second dimension
         const int n = passes - p.pass0 < 2047 ? passes - p.pass0 : 2047;
@@ -584,9 +497,9 @@ cudaError_t launch_mb(const Q4Args& a, cudaStream_t st) {
         const int slices = (p.h * p.steps + 15) / 16;  // 16 blocks of K a block: two a warp
         q4_parts_kernel<T><<<dim3(slices, rows), 256, 0, st>>>(a, p);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)grid, n);
+        cfg.gridDim = dim3((unsigned)p.grid, n);
         cfg.blockDim = dim3(Q4_THREADS);
-        cfg.dynamicSmemBytes = smem;
+        cfg.dynamicSmemBytes = p.smem;
         cfg.stream = st;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -694,7 +607,7 @@ using namespace rk;
 
 extern "C" size_t rk_linear_q4_workspace_size(int rows, int n, int k, int group, int dtype) {
     if (!size_ok(rows, 0) || !size_ok(n, 1) || !size_ok(k, 1) || !group_ok(group) || !dtype_ok(dtype)) return 0;
-    return rows ? workspace_bytes(rows, k, group, dtype) : 0;
+    return rows ? q4_workspace(rows, k, group, dtype_bytes(dtype)) : 0;
 }
 
 extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
@@ -716,7 +629,7 @@ extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, l
     if (!aligned(w, 16) || (n > 1 && (ldw % 16 || ldw < row_bytes)))
         return fail(RK_ERR_CANNOT_IMPLEMENT,
                     "rk_linear_q4: weight rows hold ceil(k / 32) x 16 bytes and start on 16-byte boundaries");
-    if (!workspace || workspace_size < workspace_bytes(rows, k, group, dtype) || !aligned(workspace, 256))
+    if (!workspace || workspace_size < q4_workspace(rows, k, group, e) || !aligned(workspace, 256))
         return fail(RK_ERR_WORKSPACE, "rk_linear_q4: workspace too small or not 256-byte aligned");
     Q4Args a{x, static_cast<const uint8_t*>(w), scales, zeros, bias, residual, y, ldx, ldw, ldr, ldy, rows, n, k,
              group, (int)(((long long)k + group - 1) / group), scale_dtype,
