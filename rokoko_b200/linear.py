@@ -28,6 +28,7 @@ from . import lib
 
 DTYPES = {torch.float32: lib.RK_DTYPE_F32, torch.float16: lib.RK_DTYPE_F16, torch.bfloat16: lib.RK_DTYPE_BF16}
 Q8 = torch.float8_e4m3fn
+MOST = 1 << 30  # rows, columns and groups: the entry points take 32-bit sizes, and ctypes would cut larger ones short
 
 
 # The current stream of a device as a plain number: the same as torch.cuda.current_stream(i).cuda_stream, without the
@@ -111,6 +112,8 @@ def _activation(x, name: str = "x"):
         raise ValueError(f"{name}: 2-D tensor expected, got {len(shape)}-D")
     if shape[1] < 1:
         raise ValueError(f"{name}: at least one column")
+    if shape[0] > MOST or shape[1] > MOST:
+        raise ValueError(f"{name}: at most 2^30 rows and columns, got {tuple(shape)}")
     return dt, dev, shape[0], shape[1]
 
 
@@ -233,6 +236,8 @@ def linear_q8(x, x_scale, w, w_scale, bias=None, residual=None, dtype=torch.floa
         raise ValueError("x: at least one column")
     if not (n >= 1 and w.shape[1] == k):
         raise ValueError(f"w: expected {k} columns and at least one row, got {tuple(w.shape)}")
+    if rows > MOST or n > MOST or k > MOST:
+        raise ValueError(f"x and w: at most 2^30 rows and columns, got {tuple(x.shape)} and {tuple(w.shape)}")
     px, ldx = _q8_operand(x, "x", dev, rows, k)
     pw, ldw = _q8_operand(w, "w", dev, n, k)
     sx = _vector(x_scale, "x_scale", torch.float32, dev, rows)
@@ -248,13 +253,13 @@ def _q4_workspace(rows: int, n: int, k: int, group: int, dt: int) -> int:
 
 
 def _check_group(group) -> None:
-    if not (group in (32, 64) or (group >= 128 and group % 128 == 0)):
-        raise ValueError(f"group: 32, 64 or a multiple of 128 expected, got {group}")
+    if not (group in (32, 64) or (128 <= group <= MOST and group % 128 == 0)):
+        raise ValueError(f"group: 32, 64 or a multiple of 128 up to 2^30 expected, got {group}")
 
 
 def quantize_q4(w, group: int = 128, zeros: bool = False, scale_dtype=torch.float32):
     """4-bit weights of w [n, k]: (codes uint8 [n, ceil(k / 32) * 16], scales [n, groups], zero points uint8 [n, groups] or
-    None).  `group` is 32, 64 or a multiple of 128."""
+    None).  `group` is 32, 64 or a multiple of 128 up to 2^30."""
     dt, dev, n, k = _activation(w, "w")
     if not (scale_dtype in DTYPES):
         raise ValueError(f"scale_dtype: float32, float16 or bfloat16 expected, got {scale_dtype}")
@@ -285,6 +290,8 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
     n, groups, row_bytes = w.shape[0], -(-k // group), (k + 31) // 32 * 16
     if not (n >= 1 and w.shape[1] == row_bytes):
         raise ValueError(f"w: expected {row_bytes} bytes a row and at least one row, got {tuple(w.shape)}")
+    if n > MOST:
+        raise ValueError(f"w: at most 2^30 rows, got {n}")
     ldw, pw = _rows(w, "w", torch.uint8, dev, n, row_bytes), w.data_ptr()
     if not (pw % 16 == 0 and (n == 1 or ldw % 16 == 0)):
         raise ValueError("w: rows start on 16-byte boundaries")

@@ -141,6 +141,17 @@ def test_python_front_end_refuses_host_tensors():
         linear.rms_norm(x.double(), w)
 
 
+def test_sizes_past_32_bits_are_refused_and_not_cut_short():
+    """2^32 + 128 reaches a 32-bit argument as 128: a group that the scales were not made for."""
+    pytest.importorskip("torch")
+    from rokoko_b200 import linear
+    for group in (32, 64, 128, 384, 1 << 30):
+        linear._check_group(group)
+    for group in ((1 << 32) + 32, (1 << 32) + 64, (1 << 32) + 128, (1 << 30) + 128, 1 << 31):
+        with pytest.raises(ValueError, match="group"):
+            linear._check_group(group)
+
+
 def test_overlapping_rows():
     """Which rows the front end takes to share memory, against the sets of their elements."""
     torch = pytest.importorskip("torch")

@@ -577,6 +577,27 @@ def test_refusals(lin):
         lin.quantize_q4(x, 100)
 
 
+def test_sizes_past_32_bits_are_refused(lin):
+    """2^32 rows reach a 32-bit argument as none: the call would return whatever its output's memory held."""
+    d = torch.device("cuda:0")
+    x = torch.empty((1 << 32, 1), dtype=F16, device=d)
+    w = torch.ones(1, dtype=F16, device=d)
+    for f in (lambda: lin.rms_norm(x, w), lambda: lin.rms_norm_q8(x, w), lambda: lin.quantize_q8(x),
+              lambda: lin.quantize_q4(x)):
+        with pytest.raises(ValueError, match="2\\^30"):
+            f()
+    del x
+    wide = torch.empty((1, (1 << 32) + 64), dtype=torch.uint8, device=d)
+    small = torch.zeros((1, 64), device=d)
+    q, s = wide.view(lin.Q8), torch.ones(1, device=d)
+    with pytest.raises(ValueError, match="2\\^30"):
+        lin.linear_q8(q, s, q, s)
+    with pytest.raises(ValueError, match="group"):
+        lin.linear_q4(small, wide[:, :32], s[:, None], (1 << 32) + 128)
+    with pytest.raises(ValueError, match="group"):
+        lin.quantize_q4(small, (1 << 32) + 128)
+
+
 def test_outputs_that_overlap_inputs_are_refused(lin):
     """Rows are worked on side by side, so an output may share memory with an input only row on row."""
     g = gen(9)
