@@ -6,30 +6,33 @@
 // Byte j of a weight row holds columns 2j (low half) and 2j + 1 (high half).
 //
 // The product runs on tcgen05 (kind::f8f6f4) without rounding anything of x or
-// of the weights.  A code 0..15 alone in a byte is an e4m3 number already: it
-// reads q 2^-9, so a word of eight codes becomes two words of operand in three
-// instructions.  x is scaled by a power of two, the same for a row, and split
-// into e5m2 parts, each sixteen times finer than the one before: three hold
-// the 8 and 11 bits of bfloat16 and half, six the 24 of float.  The parts are
-// columns of the MMA's N side; a group's accumulators are read back, put
-// together and scaled in 32 bits, less z times the group's sum of x:
+// of the weights.  A whole number up to 16 in a byte, with a sign at its top, is
+// an e4m3 number already: it reads 2^-9 times as much, so q - z comes out of a
+// word of codes by bytewise arithmetic (signed_codes).  The zero point is taken
+// off there and not from the sums: z sum x is rounded, and a large x whose weight
+// is zero would leave its rounding behind.  x is scaled by a power of two, the
+// same for a row, and split into e5m2 parts, each sixteen times finer than the
+// one before: three hold the 8 and 11 bits of bfloat16 and half, six the 24 of
+// float.  The parts are columns of the MMA's N side; a group's accumulators are
+// read back, put together and scaled in 32 bits:
 //
-//   sum_g s (2^9 sum_p 16^-p D_p - z X_g)
+//   sum_g s 2^9 sum_p 16^-p D_p
 //
 // Two launches.  The first (q4_parts_kernel) lays the parts out in the
-// workspace as the second wants them in shared memory, with the sums X.  The
-// second gives each SM an even share of the weight rows, at most 128, the
-// MMA's M side; a share of at most 64 (32) rows fills the 128 with 2 (4)
-// ranges of k one below the other, whose parts are N columns of their own: an
-// MMA takes 66 clocks whatever N <= 112 is, so its rows are what must not lie
-// idle.  Some warps turn codes into operands, one thread issues the MMAs, four
-// warps add up the accumulators.  The weights' bytes are read once.
+// workspace as the second wants them in shared memory.  The second gives each SM
+// an even share of the weight rows, at most 128, the MMA's M side; a share of at
+// most 64 (32) rows fills the 128 with 2 (4) ranges of k one below the other,
+// whose parts are N columns of their own: an MMA takes 66 clocks whatever N <=
+// 112 is, so its rows are what must not lie idle.  Some warps turn codes into
+// operands, one thread issues the MMAs, eight warps add up the accumulators.  The
+// weights' bytes are read once.
 //
 // A row with an infinity, a NaN, or magnitudes more than 2^30 apart does not fit
 // the parts; its sums are done one by one in 32 bits instead.
 #include <cuda_fp8.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "q4_plan.h"
@@ -124,28 +127,18 @@ __global__ void __launch_bounds__(256) q4_parts_kernel(const Q4Args a, const Q4P
         r.inv2 = ldexpf(1.f, back - back / 2);
         r.odd = odd;
         r.pad = 0;
-        reinterpret_cast<Q4Row*>(ws + (size_t)p.steps * p.x_stage)[m] = r;
+        reinterpret_cast<Q4Row*>(ws + (size_t)p.steps * p.x_bytes)[m] = r;
     }
     const int blocks = p.h * p.steps;
-    const int per = 16 / p.sub;  // threads whose columns make a group
-    // whole warps walk two blocks of K at a time, so that the sums' shuffles find every lane
-    for (int b0 = blockIdx.x * 2 + warp * 2 * gridDim.x; b0 < blocks; b0 += 16 * gridDim.x) {
-        const int b = b0 + (lane >> 4), g8 = lane & 15;
+    // two blocks of K a warp at a time
+    for (int b = blockIdx.x * 2 + warp * 2 * gridDim.x + (lane >> 4); b < blocks; b += 16 * gridDim.x) {
+        const int g8 = lane & 15;
         float v[8];
-        const long long c = (long long)b * Q4_KB + g8 * 8;
-        float sum = 0.f;
-        if (b < blocks) {
-            load8(c, v);
+        load8((long long)b * Q4_KB + g8 * 8, v);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = odd ? 0.f : v[i] * scale;
-            sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-        }
-        for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (b >= blocks) continue;
+        for (int i = 0; i < 8; i++) v[i] = odd ? 0.f : v[i] * scale;
         const int range = b / p.steps, step = b - range * p.steps;
-        uint8_t* st = ws + (size_t)step * p.x_stage;
-        if (g8 % per == 0)
-            reinterpret_cast<float*>(st + p.x_bytes)[(range * p.sub + g8 / per) * p.mq + m] = sum;
+        uint8_t* st = ws + (size_t)step * p.x_bytes;
 #pragma unroll
         for (int q = 0; q < PARTS; q++) {
             uint32_t w[2] = {0, 0};
@@ -168,6 +161,15 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
+}
+
+// Four codes 0..15 in a word's bytes, z in each byte of `z`: q - z in e4m3, times 2^-9.  The bytes of u + 0x80 - z never
+// carry and keep the top bit where q >= z, which the sign is the inverse of.  (The negative side by complement and the
+// increments by mask, without vabsdiff4: two more instructions, 78 us for 75 at 4 x 16384 x 16384.)
+__device__ __forceinline__ uint32_t signed_codes(uint32_t u, uint32_t z) {
+    uint32_t size;
+    asm("vabsdiff4.u32.u32.u32 %0, %1, %2, %3;" : "=r"(size) : "r"(u), "r"(z), "r"(0));
+    return size | (~(u + (0x80808080u - z)) & 0x80808080u);
 }
 
 // 32 lanes x 4 columns, not waited for
@@ -230,8 +232,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
         for (; i < p.steps; i++) {
             if (!mbar_wait_warp(&empty[s], parity, &q4_err, RK_DEV_TIMEOUT_EMPTY)) { lost = 1; break; }
             if (elect_one()) {
-                mbar_arrive_expect_tx(&full[s], p.x_stage);
-                bulk_copy(ring + s * stage + Q4_A_BYTES, ws + (size_t)i * p.x_stage, p.x_stage, &full[s]);
+                mbar_arrive_expect_tx(&full[s], p.x_bytes);
+                bulk_copy(ring + s * stage + Q4_A_BYTES, ws + (size_t)i * p.x_bytes, p.x_bytes, &full[s]);
             }
             if (++s == p.stages) { s = 0; parity ^= 1; }
         }
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
             block0[e] = range * p.steps;
         }
         uint32_t s_raw[2][SUB], z_raw[2][SUB];
+        const uint32_t pick = (SUB == 4 ? u : SUB == 2 ? u >> 1 : 0) * 0x1111u;  // the group of this lane's columns
         auto fetch = [&](int step) {                                             // converted only when they are used
 #pragma unroll
             for (int e = 0; e < 2; e++)
@@ -311,9 +314,9 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
                     const uint32_t block = block0[e] + step;
                     const uint32_t g = SUB == 1 && per > 1 ? block / per : block * SUB + b;
                     const size_t at = sz[e] + min(g, a.groups - 1u);             // past the last group x is zero
+                    z_raw[e][b] = a.z ? a.z[at] : Q4_ZERO;
                     s_raw[e][b] = a.s_dtype == RK_DTYPE_F32 ? static_cast<const uint32_t*>(a.s)[at]
                                                             : static_cast<const uint16_t*>(a.s)[at];
-                    z_raw[e][b] = a.z ? a.z[at] : Q4_ZERO;
                 }
         };
         uint4 w[8] = {};
@@ -338,16 +341,33 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
             alive = __all_sync(0xffffffffu, mbar_wait(&empty[s], parity, &q4_err, RK_DEV_TIMEOUT_EMPTY));
             if (!alive) break;
             uint8_t* st = ring + s * stage;
+            auto turn = [&](auto own) {  // own: the weights have zero points
+                uint32_t zeros[2] = {};  // of this lane's two rows, a byte a group
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint4 c = w[j];
-                constexpr uint32_t M = 0x0f0f0f0fu;
-                uint8_t* to = st + j * 1024;
-                // the second 16 bytes' place differs from the first's in the swizzled chunk's lowest bit
-                *reinterpret_cast<uint4*>(to + dst) = make_uint4(c.x & M, c.x >> 4 & M, c.y & M, c.y >> 4 & M);
-                *reinterpret_cast<uint4*>(to + (dst ^ 16)) = make_uint4(c.z & M, c.z >> 4 & M, c.w & M, c.w >> 4 & M);
-                load(j, i + STRIDE, m);
-            }
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int b = 0; b < SUB; b++) zeros[e] |= z_raw[e][b] << (8 * b);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint4 c = w[j];
+                    constexpr uint32_t M = 0x0f0f0f0fu;
+                    uint8_t* to = st + j * 1024;
+                    uint32_t z = Q4_ZERO * 0x01010101u;
+                    if constexpr (decltype(own)::value) {
+                        z = __shfl_sync(0xffffffffu, zeros[j >> 2], (lane >> 2) + 8 * (j & 3));
+                        asm("prmt.b32 %0, %0, %0, %1;" : "+r"(z) : "r"(pick));
+                    }
+                    // the second 16 bytes' place differs from the first's in the swizzled chunk's lowest bit
+                    *reinterpret_cast<uint4*>(to + dst) = make_uint4(signed_codes(c.x & M, z), signed_codes(c.x >> 4 & M, z),
+                                                                     signed_codes(c.y & M, z), signed_codes(c.y >> 4 & M, z));
+                    *reinterpret_cast<uint4*>(to + (dst ^ 16)) =
+                        make_uint4(signed_codes(c.z & M, z), signed_codes(c.z >> 4 & M, z), signed_codes(c.w & M, z),
+                                   signed_codes(c.w >> 4 & M, z));
+                    load(j, i + STRIDE, m);
+                }
+            };
+            if (a.z) turn(std::true_type{});
+            else turn(std::false_type{});
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
@@ -356,9 +376,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
                     const float f = a.s_dtype == RK_DTYPE_F32 ? __uint_as_float(r)
                                     : a.s_dtype == RK_DTYPE_F16 ? __half2float(__ushort_as_half((uint16_t)r))
                                                                 : __uint_as_float(r << 16);
-                    // 2^-9 is left to the end, so the zero point comes in at 2^-9
-                    reinterpret_cast<float2*>(st + p.s_off)[(half + e * 32 + lane) * SUB + b] =
-                        make_float2(f, (float)z_raw[e][b] * (1.f / 512.f));
+                    reinterpret_cast<float*>(st + p.s_off)[(half + e * 32 + lane) * SUB + b] = f;
                 }
             if (i + STRIDE < p.steps) fetch(i + STRIDE);
             // Orders these plain writes before the MMAs' reads: here, where there is time, and not in the issuing thread.
@@ -387,29 +405,26 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
         for (int step = SUB == 1 ? set : 0; step < p.steps && alive; step += TURN) {
             alive = __all_sync(0xffffffffu, mbar_wait(&full[s], parity, &q4_err, RK_DEV_TIMEOUT_FULL));
             if (!alive) break;
-            const float* xs = reinterpret_cast<const float*>(ring + s * stage + Q4_A_BYTES + p.x_bytes) + range * SUB * p.mq;
-            const float2* sz = reinterpret_cast<const float2*>(ring + s * stage + p.s_off) + i * SUB;
+            const float* scales = reinterpret_cast<const float*>(ring + s * stage + p.s_off) + i * SUB;
 #pragma unroll 1
             for (int b = SUB == 1 ? 0 : set; b < SUB; b += 2) {
                 alive = __all_sync(0xffffffffu, mbar_wait(&d_full[d], d_parity, &q4_err, RK_DEV_TIMEOUT_ACC));
                 if (!alive) break;
                 tc_fence_after();
-                const float f = sz[b].x, z = sz[b].y;
+                const float f = scales[b];
 #pragma unroll
                 for (int m = 0; m < MB; m += 4) {
                     if (m < p.mq) {
                         float v[PARTS][4];
 #pragma unroll
                         for (int q = 0; q < PARTS; q++) tmem_ld4(base + d * p.acc_cols + q * p.mq + m, v[q]);
-                        const float4 x4 = *reinterpret_cast<const float4*>(xs + b * p.mq + m);
-                        const float x[4] = {x4.x, x4.y, x4.z, x4.w};
                         tmem_ld_wait(v);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             float t = v[PARTS - 1][j];
 #pragma unroll
                             for (int q = PARTS - 2; q >= 0; q--) t = fmaf(t, 0.0625f, v[q][j]);
-                            acc[m + j] = fmaf(f, fmaf(-z, x[j], t), acc[m + j]);
+                            acc[m + j] = fmaf(f, t, acc[m + j]);
                         }
                     }
                 }
@@ -438,7 +453,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
     }
     if (lost) return;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the first launch's rows, here read plainly
-    const Q4Row* info = reinterpret_cast<const Q4Row*>(ws + (size_t)p.steps * p.x_stage);
+    const Q4Row* info = reinterpret_cast<const Q4Row*>(ws + (size_t)p.steps * p.x_bytes);
     for (int m = 0; m < rows; m++) {
         const Q4Row r = info[m];
         if (!r.odd) {
@@ -607,7 +622,7 @@ using namespace rk;
 
 extern "C" size_t rk_linear_q4_workspace_size(int rows, int n, int k, int group, int dtype) {
     if (!size_ok(rows, 0) || !size_ok(n, 1) || !size_ok(k, 1) || !group_ok(group) || !dtype_ok(dtype)) return 0;
-    return rows ? q4_workspace(rows, k, group, dtype_bytes(dtype)) : 0;
+    return rows ? q4_workspace(rows, k, dtype_bytes(dtype)) : 0;
 }
 
 extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
@@ -629,7 +644,7 @@ extern "C" rk_status rk_linear_q4(const void* x, long long ldx, const void* w, l
     if (!aligned(w, 16) || (n > 1 && (ldw % 16 || ldw < row_bytes)))
         return fail(RK_ERR_CANNOT_IMPLEMENT,
                     "rk_linear_q4: weight rows hold ceil(k / 32) x 16 bytes and start on 16-byte boundaries");
-    if (!workspace || workspace_size < q4_workspace(rows, k, group, e) || !aligned(workspace, 256))
+    if (!workspace || workspace_size < q4_workspace(rows, k, e) || !aligned(workspace, 256))
         return fail(RK_ERR_WORKSPACE, "rk_linear_q4: workspace too small or not 256-byte aligned");
     Q4Args a{x, static_cast<const uint8_t*>(w), scales, zeros, bias, residual, y, ldx, ldw, ldr, ldy, rows, n, k,
              group, (int)(((long long)k + group - 1) / group), scale_dtype,

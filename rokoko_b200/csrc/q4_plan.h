@@ -34,9 +34,9 @@ struct Q4Plan {
     int mq;              // activation rows of a pass, in fours
     int nc;              // N columns of a range: parts x mq, in eights
     int mma_n;           // N of an MMA
-    uint32_t x_bytes, x_stage;  // of a step: the operand rows [h * nc][128] and after them the sums [h][sub][mq]
+    uint32_t x_bytes;    // of a step: the operand rows [h * nc][128]
     int stages;
-    uint32_t s_off, stage;      // shared memory: [128][sub] scales and zero points of a stage, a stage
+    uint32_t s_off, stage;      // shared memory: [128][sub] scales of a stage, a stage
     uint32_t acc_cols, tmem_cols, idesc;
     int accs;                   // accumulators: 4 where they fit, 2
     size_t pass_bytes;   // workspace of a pass
@@ -55,12 +55,12 @@ inline void q4_widths(int rows, size_t type_bytes, int& mq, int& nc) {
     nc = (q4_parts(type_bytes) * mq + 7) / 8 * 8;
 }
 
-inline size_t q4_workspace(int rows, int k, int group, size_t type_bytes) {
+inline size_t q4_workspace(int rows, int k, size_t type_bytes) {
     const long long passes = ((long long)rows + Q4_ROWS - 1) / Q4_ROWS, blocks = ((long long)k + Q4_KB - 1) / Q4_KB;
     int mq, nc;
     q4_widths(rows, type_bytes, mq, nc);
     // 4 even ranges of k have up to 3 blocks more than k
-    const size_t pass = (size_t)(blocks + 3) * ((size_t)nc * 128 + (size_t)q4_sub(group) * mq * 4) + Q4_ROWS * sizeof(Q4Row);
+    const size_t pass = (size_t)(blocks + 3) * nc * 128 + Q4_ROWS * sizeof(Q4Row);
     return (size_t)passes * ((pass + 255) / 256 * 256);
 }
 
@@ -81,16 +81,15 @@ inline bool q4_plan(int rows, int n, int k, int group, size_t type_bytes, int sm
     p.steps = (blocks + p.h - 1) / p.h;
     p.sub = q4_sub(group);
     p.x_bytes = (uint32_t)(p.h * p.nc * 128);
-    p.x_stage = p.x_bytes + (uint32_t)(p.h * p.sub * p.mq * 4);
     p.mma_n = (p.h * p.nc + 15) / 16 * 16;
     p.acc_cols = (uint32_t)(p.mma_n + 31) / 32 * 32;
     p.accs = 4 * p.acc_cols <= 512 ? 4 : 2;
     p.tmem_cols = 32;
     while (p.tmem_cols < p.accs * p.acc_cols) p.tmem_cols *= 2;
-    p.pass_bytes = ((size_t)p.steps * p.x_stage + Q4_ROWS * sizeof(Q4Row) + 255) / 256 * 256;
+    p.pass_bytes = ((size_t)p.steps * p.x_bytes + Q4_ROWS * sizeof(Q4Row) + 255) / 256 * 256;
     // an MMA of N in sixteens may read eight rows past a stage's operand rows, which the scales' place makes up for
-    p.s_off = Q4_A_BYTES + (p.x_stage + 127) / 128 * 128;
-    p.stage = (p.s_off + Q4_M * p.sub * 2 * (uint32_t)sizeof(float) + 1023) / 1024 * 1024;
+    p.s_off = Q4_A_BYTES + p.x_bytes;
+    p.stage = (p.s_off + Q4_M * p.sub * (uint32_t)sizeof(float) + 1023) / 1024 * 1024;
     p.stages = (Q4_SMEM - 1024) / (int)p.stage;
     if (p.stages > Q4_STAGES) p.stages = Q4_STAGES;
     // A wait tells a stage's rounds apart by one bit, so no warp may come to a stage's barrier two rounds early.  A warp

@@ -5,7 +5,7 @@ extern "C" int q4_plan_of(int rows, int n, int k, int group, int type_bytes, int
     rk::Q4Plan p;
     if (!rk::q4_plan(rows, n, k, group, (size_t)type_bytes, sms, p)) return 0;
     const long long v[] = {p.stages, p.accs, p.sub, p.steps, p.smem, (long long)p.pass_bytes, p.grid, p.tmem_cols,
-                           (long long)rk::q4_workspace(rows, k, group, (size_t)type_bytes)};
+                           (long long)rk::q4_workspace(rows, k, (size_t)type_bytes)};
     for (int i = 0; i < 9; i++) out[i] = v[i];
     return 1;
 }

@@ -379,6 +379,27 @@ def test_linear_q4_uneven_magnitudes(lin, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True], ids=["sym", "zeros"])
+def test_linear_q4_large_values_at_the_zero_point(lin, dtype, group, zeros):
+    """One value of a row up to 2^29 times the others, where every weight is zero (its code is the zero point): it has
+    no part in sum |x w|, so nothing of it may show."""
+    g, rows, n, k = gen(18), 40, 150, 512
+    spread = torch.tensor([0, 10, 13, 15] if dtype == F16 else [0, 10, 13, 17, 21, 25, 29], device="cuda").double()
+    x = (torch.rand(rows, k, generator=g, device="cuda") * 1.5 + 0.5) * randn(g, rows, k).sign()
+    w, s, z = q4_case(g, n, k, group, F32, zeros)
+    for at in (5, k - 2):  # one in a high half of a byte, one in a low half
+        x[:, at] = torch.exp2(spread[torch.arange(rows, device="cuda") % len(spread)]).float()
+        code = z[:, at // group] if zeros else torch.full((n,), 8, dtype=torch.uint8, device="cuda")
+        low, high = w[:, at // 2] & 15, w[:, at // 2] >> 4
+        w[:, at // 2] = code | high << 4 if at % 2 == 0 else low | code << 4
+    x = x.to(dtype)
+    for r in (3, rows):
+        ref, err = q4_ref(x[:r], w, s, z, group, None, None)
+        close(lin.linear_q4(x[:r], w, s, group, zeros=z), ref, err, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_linear_q4_strides_pads_and_in_place(lin, dtype):
     g, rows, n, k = gen(13), 5, 45, 250
     x = randn(g, rows, k, dtype=dtype)
