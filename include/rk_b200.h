@@ -183,10 +183,13 @@ RK_API rk_status rk_linear_q8(const void* x, long long ldx, const float* x_scale
  * span [min(w, 0), max(w, 0)] of the group, else scale = max|w| / 7; w must be
  * finite.
  * rk_linear_q4: y[rows][n] = x w^T + bias + residual, x and y of type dtype
- * (32-bit x keeps its precision: x is split into 8-bit parts that hold all of
- * it; scales below 2^90), bias float or NULL, residual in y's type or NULL (may be y itself).  Meant for few
- * rows, where the weights' bytes are the cost; any number of rows is right, and
- * beyond a few dozen rk_linear_q8 or the conv seam are faster. */
+ * (x is split into 8-bit parts, which hold 16-bit x exactly and 32-bit x but for
+ * its last bit; scales below 2^90), bias float or NULL, residual in y's type or
+ * NULL (may be y itself).  Meant for few rows, where the weights' bytes are the
+ * cost; any number of rows is right, and beyond a few dozen rk_linear_q8 or the
+ * conv seam are faster.  A row of x with a nonzero value more than 2^30 times
+ * (half: 2^27 times) smaller than its largest, an infinity or a NaN does not fit
+ * the parts and is worked on by plain sums, which take far longer. */
 RK_API rk_status rk_quantize_q4(const void* w, long long ldw, void* q, long long ldq, void* scales, uint8_t* zeros,
                                 int n, int k, int group, int dtype, int scale_dtype, void* stream);
 RK_API rk_status rk_linear_q4(const void* x, long long ldx, const void* w, long long ldw, const void* scales,

@@ -5,16 +5,17 @@
 //
 // Byte j of a weight row holds columns 2j (low half) and 2j + 1 (high half).
 //
-// The product runs on tcgen05 (kind::f8f6f4) without rounding anything of x or
-// of the weights.  A whole number up to 16 in a byte, with a sign at its top, is
-// an e4m3 number already: it reads 2^-9 times as much, so q - z comes out of a
-// word of codes by bytewise arithmetic (signed_codes).  The zero point is taken
-// off there and not from the sums: z sum x is rounded, and a large x whose weight
-// is zero would leave its rounding behind.  x is scaled by a power of two, the
-// same for a row, and split into e5m2 parts, each sixteen times finer than the
-// one before: three hold the 8 and 11 bits of bfloat16 and half, six the 24 of
-// float.  The parts are columns of the MMA's N side; a group's accumulators are
-// read back, put together and scaled in 32 bits:
+// The product runs on tcgen05 (kind::f8f6f4) without rounding anything of the
+// weights, or of x in 16 bits.  A whole number up to 16 in a byte, with a sign at
+// its top, is an e4m3 number already: it reads 2^-9 times as much, so q - z comes
+// out of a word of codes by bytewise arithmetic (signed_codes).  The zero point is
+// taken off there and not from the sums: z sum x is rounded, and a large x whose
+// weight is zero would leave its rounding behind.  x is scaled by a power of two,
+// the same for a row, and split into e5m2 parts, each sixteen times finer than the
+// one before: three hold the 8 and 11 bits of bfloat16 and half, six 23 of the 24
+// of float (Q4Type says how far below a row's largest).  The parts are columns of
+// the MMA's N side; a group's accumulators are read back, put together and scaled
+// in 32 bits:
 //
 //   sum_g s 2^9 sum_p 16^-p D_p
 //
@@ -27,8 +28,8 @@
 // operands, one thread issues the MMAs, eight warps add up the accumulators.  The
 // weights' bytes are read once.
 //
-// A row with an infinity, a NaN, or magnitudes more than 2^30 apart does not fit
-// the parts; its sums are done one by one in 32 bits instead.
+// A row with an infinity, a NaN, or magnitudes too far apart does not fit the
+// parts; its sums are done one by one in 32 bits instead.
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -44,8 +45,13 @@ namespace {
 
 constexpr int Q4_ZERO = 8;  // the zero point of weights that have none of their own
 
-template <typename T> struct Q4Type { static constexpr int PARTS = 3; };
-template <> struct Q4Type<float> { static constexpr int PARTS = 6; };
+// The parts of a type, and how many binades below its row's largest magnitude a value may lie to be left to them.  The
+// parts' last place is 2^-24 with three and 2^-36 with six where the largest lies in [2^13, 2^14), which holds bfloat16
+// exactly down to 30 binades and half down to 27.  Of float the last place may be lost (1.6 % of values), below 27
+// binades up to 8 of it: 16 u of a value (u = 2^-24), half of what the sums' last roundings are allowed.
+template <typename T> struct Q4Type { static constexpr int PARTS = 3, SPAN = 30; };
+template <> struct Q4Type<__half> { static constexpr int PARTS = 3, SPAN = 27; };
+template <> struct Q4Type<float> { static constexpr int PARTS = 6, SPAN = 30; };
 
 struct Q4Args {
     const void* x;
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(256) q4_parts_kernel(const Q4Args a, const Q4P
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) { top = max(top, sh_max[i]); low = min(low, sh_min[i]); }
-    const bool odd = top == 255 || (low < 255 && low < top - 30);
+    const bool odd = top == 255 || (low < 255 && low < top - Q4Type<T>::SPAN);
     // the largest magnitude comes to lie in [2^13, 2^14): e5m2 ends at 57344
     const int shift = min(126, 13 - (top - 127));
     const float scale = odd ? 0.f : __uint_as_float((uint32_t)(shift + 127) << 23);

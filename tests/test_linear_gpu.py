@@ -400,6 +400,26 @@ def test_linear_q4_large_values_at_the_zero_point(lin, dtype, group, zeros):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("binades", [26, 27, 28, 29, 30, 31])
+def test_linear_q4_small_values_keep_their_bits(lin, dtype, binades):
+    """Values that far below their row's largest, which meets a weight of zero: the small ones alone are the result.
+    Parts of 32-bit x may lose 8 last places of a value, 16 u of it and so of sum |x w|; the bound of `linear` has 32 u
+    beside its K / 4 u for the last roundings, of which there are fewer than 8."""
+    g, rows, n, k = gen(19), 4, 80, 32
+    if dtype == F16 and binades > 29:
+        pytest.skip("half has no normal numbers so far apart")
+    top = 2.0 ** (15 if dtype == F16 else 40)
+    x = (torch.rand(rows, k, generator=g, device="cuda", dtype=torch.float64) * 0.99 + 1) * top * 2.0 ** -binades
+    x = x.to(dtype) * randn(g, rows, k).sign().to(dtype)
+    x[:, 7] = top
+    w, s, _ = q4_case(g, n, k, 32, F32, False)
+    w[:, 3] = 8 << 4 | w[:, 3] & 15
+    s *= 1024.0  # results beyond half's smallest numbers
+    ref, err = q4_ref(x, w, s, None, 32, None, None)
+    close(lin.linear_q4(x, w, s, 32), ref, err, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_linear_q4_strides_pads_and_in_place(lin, dtype):
     g, rows, n, k = gen(13), 5, 45, 250
     x = randn(g, rows, k, dtype=dtype)
