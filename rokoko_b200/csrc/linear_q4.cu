@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
                 for (int k = lane; k < a.k; k += 32) {
                     const size_t g = (size_t)n * a.groups + k / a.group;
                     const int q = (w[k >> 1] >> (k & 1) * 4 & 15) - (a.z ? a.z[g] : Q4_ZERO);
-                    v += load_as_f32(a.s, g, a.s_dtype) * ((float)q * to_f32(x[k]));
+                    v += (load_as_f32(a.s, g, a.s_dtype) * (float)q) * to_f32(x[k]);  // q x may pass the largest float
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

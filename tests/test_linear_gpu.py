@@ -419,6 +419,24 @@ def test_linear_q4_small_values_keep_their_bits(lin, dtype, binades):
     close(lin.linear_q4(x, w, s, 32), ref, err, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -20], ids=["even", "uneven"])
+def test_linear_q4_values_near_the_largest_float(lin, dtype, small):
+    """A value that passes the largest float when it is multiplied by its code, and not when by its weight."""
+    g = gen(21)
+    x = randn(g, 3, 96, dtype=dtype) * small
+    x[1] = 2.0 ** 100
+    x[1, 3] = 2.0 ** 126
+    if small != 1:
+        x[1, 50] = small
+    w, s, z = q4_case(g, 70, 96, 32, F32, True)
+    w[:, 1] = 0xf0 | w[:, 1] & 15
+    z[:, 0] = 0
+    ref, err = q4_ref(x, w, s, z, 32, None, None)
+    assert torch.isfinite(ref.float()).all()
+    close(lin.linear_q4(x, w, s, 32, zeros=z), ref, err, dtype)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_linear_q4_strides_pads_and_in_place(lin, dtype):
     g, rows, n, k = gen(13), 5, 45, 250
