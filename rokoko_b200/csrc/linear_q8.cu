@@ -80,7 +80,8 @@ __device__ __forceinline__ void store_rows(const Q8Args& a, long long m, int n, 
         const float f[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v = fmaf(acc[j + i], f[i] * sw, bias);
+            // one scale after the other: their product may leave float's range where the result does not
+            float v = fmaf(acc[j + i] * sw, f[i], bias);
             if (a.res && (FULL || j + i < left)) v += to_f32(rv[j + i]);
             if (FULL || j + i < left) *y = from_f32<T>(v);
             y += a.ldy;

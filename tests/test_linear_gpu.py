@@ -268,6 +268,26 @@ def test_linear_q8_strides_pads_and_in_place(lin, rows, dtype):
     assert (by[:, :13] == 7).all() and (by[:, 13 + n:] == 7).all()
 
 
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear_q8_scales_whose_product_is_out_of_range(lin, rows, bias):
+    """Scales whose product is smaller than float's normal numbers or passes its largest, and results that do neither."""
+    g, n, k = gen(22), 70, 2048
+    bias = randn(g, n) * 1e-36 if bias else None
+    x, sx = lin.quantize_q8(randn(g, rows, k) * 1e-22)
+    w, sw = lin.quantize_q8(randn(g, n, k) * 1e-16)
+    assert float(sx.max() * sw.max()) < 2.0 ** -126
+    ref, err = q8_ref(x, sx, w, sw, bias, None)
+    close(lin.linear_q8(x, sx, w, sw, bias=bias), ref, err, F32)
+    big, small = torch.zeros(rows, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    big[:, ::2], small[:, 1::2] = 1e30, 1e20  # what one has is zero in the other
+    x, sx = lin.quantize_q8(big)
+    w, sw = lin.quantize_q8(small)
+    sw = sw * 1e5
+    assert torch.isinf(sx[0] * sw[0])
+    assert (lin.linear_q8(x, sx, w, sw) == 0).all()
+
+
 def test_linear_q8_nan_and_infinity_stay_in_their_row(lin):
     g = gen(10)
     for rows in (6, 200):
