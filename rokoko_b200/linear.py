@@ -15,14 +15,15 @@ the current stream of the inputs' device, or the ones that `out` and `sum_out`
 name; these may be an input itself where a function says so and otherwise share
 no memory with x, the residual or each other.  Arguments that do not fit raise
 ValueError before anything is enqueued.  The operators are for serving and have
-no gradients: an input that requires one is refused while gradients are
-recorded.  There is no other path than librokoko_b200.so.
+no gradients: an input that requires one while gradients are recorded, or carries
+a forward-mode tangent, is refused.  There is no other path than librokoko_b200.so.
 """
 from __future__ import annotations
 
 import functools
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import lib
 
@@ -42,16 +43,24 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _place(t, name: str, dtype, dev: int) -> None:
-    """Raises for what _rows and _vector found not to be a tensor of this type on this device."""
+    """Raises for what _odd found, where it is not a tensor of this type on this device or not to be read as it lies."""
     _need(isinstance(t, torch.Tensor), f"{name}: a tensor is expected")
     _need(t.get_device() == dev, f"{name}: expected a tensor on cuda:{dev}, got {t.device}")
     _need(t.dtype is dtype, f"{name}: expected {dtype}, got {t.dtype}")
     _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient; this operator has none")
+    _need(forward_ad.unpack_dual(t).tangent is None, f"{name} carries a tangent; this operator has no derivatives")
+    _need(not t.is_neg(), f"{name}: a view of negated values; resolve_neg() makes a tensor of them")
+
+
+def _odd(t, dtype, dev: int) -> bool:
+    """Whether _place has to look at it: anything but plain values in the memory of this device."""
+    return (t.__class__ is not torch.Tensor or t.dtype is not dtype or t.get_device() != dev or t.requires_grad or
+            forward_ad._current_level >= 0 or t.is_neg())
 
 
 def _rows(t, name: str, dtype, dev: int, rows: int, cols: int) -> int:
     """Checks a [rows, cols] tensor of this type on this device and returns its row stride in elements."""
-    if t.__class__ is not torch.Tensor or t.dtype is not dtype or t.get_device() != dev or t.requires_grad:
+    if _odd(t, dtype, dev):
         _place(t, name, dtype, dev)
     shape = t.shape
     if len(shape) != 2:
@@ -67,7 +76,7 @@ def _rows(t, name: str, dtype, dev: int, rows: int, cols: int) -> int:
 
 
 def _vector(t, name: str, dtype, dev: int, n: int) -> int:
-    if t.__class__ is not torch.Tensor or t.dtype is not dtype or t.get_device() != dev or t.requires_grad:
+    if _odd(t, dtype, dev):
         _place(t, name, dtype, dev)
     if t.shape != (n,):
         raise ValueError(f"{name}: expected shape ({n},), got {tuple(t.shape)}")

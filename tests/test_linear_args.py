@@ -152,6 +152,39 @@ def test_sizes_past_32_bits_are_refused_and_not_cut_short():
             linear._check_group(group)
 
 
+def test_tensors_that_are_more_than_their_memory_are_refused():
+    """A forward-mode tangent would be dropped, a negated view be read without its sign.  (On host tensors: device -1.)"""
+    torch = pytest.importorskip("torch")
+    import torch.autograd.forward_ad as fwd
+    from rokoko_b200 import linear
+    x, v = torch.randn(3, 4), torch.randn(4)
+
+    def both(x, v):
+        linear._rows(x, "x", torch.float32, -1, 3, 4)
+        linear._vector(v, "v", torch.float32, -1, 4)
+    both(x, v)
+    with fwd.dual_level():
+        both(x, v)
+        with pytest.raises(ValueError, match="x carries a tangent"):
+            both(fwd.make_dual(x, x), v)
+        with pytest.raises(ValueError, match="v carries a tangent"):
+            both(x, fwd.make_dual(v, v))
+        with torch.no_grad(), pytest.raises(ValueError, match="x carries a tangent"):
+            both(fwd.make_dual(x, x), v)
+
+    def f(x, v):
+        with pytest.raises(ValueError, match="carries a tangent"):
+            both(x, v)
+        return x.sum()
+    torch.func.jvp(f, (x, v), (x, v))
+    with pytest.raises(ValueError, match="x requires a gradient"):
+        torch.func.grad(lambda x: both(x, v))(x)
+    z = torch.randn(3, 1, dtype=torch.complex64).conj().imag
+    with pytest.raises(ValueError, match="x: a view of negated values"):
+        linear._rows(z, "x", torch.float32, -1, 3, 1)
+    linear._rows(z.resolve_neg(), "x", torch.float32, -1, 3, 1)
+
+
 def test_overlapping_rows():
     """Which rows the front end takes to share memory, against the sets of their elements."""
     torch = pytest.importorskip("torch")
