@@ -13,7 +13,7 @@ row stride), in float32, float16 or bfloat16; what a call reads and writes
 stands at the entry points of include/rk_b200.h.  Results are new tensors on
 the current stream of the inputs' device, or the ones that `out` and `sum_out`
 name; these may be an input itself where a function says so and otherwise share
-no memory with x, the residual or each other.  Arguments that do not fit raise
+no memory with an input or each other.  Arguments that do not fit raise
 ValueError before anything is enqueued.  The operators are for serving and have
 no gradients: an input that requires one while gradients are recorded, or carries
 a forward-mode tangent, is refused.  There is no other path than librokoko_b200.so.
@@ -86,22 +86,22 @@ def _vector(t, name: str, dtype, dev: int, n: int) -> int:
 
 
 def _apart(out, other, what: str, itself: bool = False) -> None:
-    """Refuses an output that shares memory with `other`, a tensor of the same rows; `itself`: the very same rows may.
+    """Refuses an output that shares memory with `other`, a vector or a tensor of rows; `itself`: the very same rows may.
     Columns of one buffer beside each other are apart."""
-    if out is None or other is None or not out.numel():
+    if out is None or other is None or not (out.numel() and other.numel()):
         return
     a, b = out.data_ptr(), other.data_ptr()
+    na, nb = out.shape[0], other.shape[0] if other.dim() > 1 else 1
     lda, ldb = out.stride(0) * out.element_size(), other.stride(0) * other.element_size()
-    wa, wb = out.shape[1] * out.element_size(), other.shape[1] * other.element_size()
-    one = out.shape[0] == 1
-    if itself and a == b and (one or lda == ldb):
+    wa, wb = out.shape[1] * out.element_size(), other.shape[-1] * other.element_size()
+    if itself and a == b and (na == 1 or lda == ldb):
         return
-    far = 0 if one else out.shape[0] - 1
-    if a + far * lda + wa <= b or b + far * ldb + wb <= a:
+    if a + (na - 1) * lda + wa <= b or b + (nb - 1) * ldb + wb <= a:
         return
-    if not one and lda == ldb:
-        at = (b - a) % lda
-        if at >= wa and at + wb <= lda:
+    pitch = 0 if na == 1 == nb else lda if nb == 1 or na > 1 and lda == ldb else ldb if na == 1 else 0
+    if pitch:
+        at = (b - a) % pitch
+        if at >= wa and at + wb <= pitch:
             return
     raise ValueError(f"{what} overlap")
 
@@ -159,6 +159,7 @@ def _norm_args(x, weight, residual, sum_out):
         sp = sum_out.data_ptr()
         _apart(sum_out, x, "sum_out and x", itself=True)
         _apart(sum_out, residual, "sum_out and residual", itself=True)
+        _apart(sum_out, weight, "sum_out and weight")
     elif residual is not None:
         sum_out, lds = x.new_empty((rows, cols)), cols
         sp = sum_out.data_ptr()
@@ -180,6 +181,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
         _apart(out, sum_out, "out and sum_out")
         _apart(out, x, "out and x", itself=True)
         _apart(out, residual, "out and residual", itself=True)
+        _apart(out, weight, "out and weight")
     _call("rk_rms_norm", dev, *args, out.data_ptr(), ldy, rows, cols, eps, dt)
     return out if h is None else (out, h)
 
@@ -204,18 +206,21 @@ def quantize_q8(x):
     return q, scale
 
 
-def _finish_args(x, rows: int, n: int, dtype, dev: int, bias, residual, out):
+def _finish_args(rows: int, n: int, dtype, dev: int, bias, residual, out, **inputs):
+    """bias, residual and the output of a linear layer; `inputs`: by name, what else the output has to be apart from."""
     bp = _vector(bias, "bias", torch.float32, dev, n) if bias is not None else None
     rp, ldr = None, 0
     if residual is not None:
         ldr = _rows(residual, "residual", dtype, dev, rows, n)
         rp = residual.data_ptr()
     if out is None:
-        out, ldy = x.new_empty((rows, n), dtype=dtype), n
+        out, ldy = inputs["x"].new_empty((rows, n), dtype=dtype), n
     else:
         ldy = _rows(out, "out", dtype, dev, rows, n)
         _apart(out, residual, "out and residual", itself=True)
-        _apart(out, x, "out and x")
+        _apart(out, bias, "out and bias")
+        for name, t in inputs.items():
+            _apart(out, t, f"out and {name}")
     return out, (bp, rp, ldr, out.data_ptr(), ldy)
 
 
@@ -251,7 +256,7 @@ def linear_q8(x, x_scale, w, w_scale, bias=None, residual=None, dtype=torch.floa
     pw, ldw = _q8_operand(w, "w", dev, n, k)
     sx = _vector(x_scale, "x_scale", torch.float32, dev, rows)
     sw = _vector(w_scale, "w_scale", torch.float32, dev, n)
-    out, tail = _finish_args(x, rows, n, dtype, dev, bias, residual, out)
+    out, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, x_scale=x_scale, w_scale=w_scale)
     _call("rk_linear_q8", dev, px, ldx, sx, pw, ldw, sw, *tail, rows, n, k, dt)
     return out
 
@@ -318,7 +323,7 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
         if not (ldz == groups or n == 1):
             raise ValueError("zeros: a contiguous tensor is expected")
         zp = zeros.data_ptr()
-    out, tail = _finish_args(x, rows, n, dtype, dev, bias, residual, out)
+    out, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, scales=scales, zeros=zeros)
     size = _q4_workspace(rows, n, k, group, dt)
     ws = x.new_empty((size,), dtype=torch.uint8)  # torch's blocks start on 512-byte boundaries
     _call("rk_linear_q4", dev, x.data_ptr(), ldx, pw, ldw, scales.data_ptr(), zp, *tail, ws.data_ptr(), size, rows, n, k,

@@ -208,6 +208,37 @@ def test_overlapping_rows():
     _apart(buf.view(20, 20)[:, :4], buf.view(20, 20)[:, :4], "x and y", itself=True)
 
 
+def test_rows_and_vectors_that_overlap():
+    """The same for an output and a vector, of another element size too, or rows in another number."""
+    torch = pytest.importorskip("torch")
+    from rokoko_b200.linear import _apart
+    buf = torch.zeros(400)
+    seen = set()
+
+    def where(t):
+        step = t.element_size()
+        rows, pitch = (t.shape[0], t.stride(0) * step) if t.dim() > 1 else (1, 0)
+        return {t.data_ptr() + i * pitch + j for i in range(rows) for j in range(t.shape[-1] * step)}
+    for rows, cols, ld in ((1, 7, 7), (1, 4, 30), (3, 7, 16), (3, 7, 7), (3, 4, 20)):
+        out = buf.as_strided((rows, cols), (ld, 1), 100)
+        others = [buf[at:at + n] for at in range(80, 165) for n in (1, 5, 9)]
+        others += [t.view(torch.uint8) for t in others]
+        others += [buf.as_strided((r, c), (p, 1), at) for at in range(60, 165, 3) for r in (1, 2, 5) for c in (1, 9)
+                   for p in (ld, 11) if p >= c]
+        for t in others:
+            try:
+                _apart(out, t, "out and other")
+                free = True
+            except ValueError:
+                free = False
+            meet = bool(where(out) & where(t))
+            assert not (free and meet)
+            many = t.dim() > 1 and t.shape[0] > 1
+            assert free or meet or (many and rows > 1 and t.stride(0) != ld)  # in vain for unlike pitches alone
+            seen.add((free, t.dim()))
+    assert len(seen) == 4
+
+
 def test_header_constants_match():
     from rokoko_b200 import lib
     assert (lib.RK_DTYPE_F32, lib.RK_DTYPE_F16, lib.RK_DTYPE_BF16) == (F32, F16, BF16)

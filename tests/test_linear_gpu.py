@@ -711,6 +711,35 @@ def test_outputs_that_overlap_inputs_are_refused(lin):
         lin.linear_q4(one[:, :64], p4, s4, 32, out=one[:, 63:127])
 
 
+def test_outputs_that_overlap_weights_are_refused(lin):
+    """Every row reads them, so no output may share their memory, not even row on row."""
+    g = gen(23)
+    x = randn(g, 64, 64)
+    w = randn(g, 64)
+    with pytest.raises(ValueError, match="out and weight overlap"):
+        lin.rms_norm(x, x[0], out=x)
+    for f in (lin.rms_norm, lin.rms_norm_q8):
+        with pytest.raises(ValueError, match="sum_out and weight overlap"):
+            f(x, x[3], sum_out=x)
+    before = x.clone()
+    q, s = lin.quantize_q8(x)
+    bytes_ = torch.empty((64, 64 * 4), dtype=torch.uint8, device="cuda")
+    wq = bytes_[:, :64].view(lin.Q8)
+    wq.copy_(q)
+    over = bytes_.view(F32)
+    for a in (dict(w=wq, out=over), dict(w_scale=x[0], out=x), dict(x_scale=x[5], out=x), dict(bias=x[63], out=x)):
+        name = [k for k in a if k != "out"][0]
+        with pytest.raises(ValueError, match=f"out and {name} overlap"):
+            lin.linear_q8(**(dict(x=q, x_scale=s, w=q, w_scale=s) | a))
+    p4, s4, z4 = lin.quantize_q4(x, 32, zeros=True)
+    held = torch.empty((64, 64 * 4), dtype=torch.uint8, device="cuda")
+    p5, z5, s5 = held[:, 16:48], held.view(-1)[128:256].view(64, 2), held.view(F32).view(-1)[64:192].view(64, 2)
+    for a in (dict(w=p5), dict(zeros=z5), dict(scales=s5), dict(bias=held.view(F32)[2])):
+        with pytest.raises(ValueError, match=f"out and {list(a)[0]} overlap"):
+            lin.linear_q4(**(dict(x=x, w=p4, scales=s4, group=32, zeros=z4, out=held.view(F32)) | a))
+    assert torch.equal(x, before)
+
+
 def test_zero_rows(lin):
     x, w = torch.zeros(0, 64, device="cuda"), torch.ones(64, device="cuda")
     assert lin.rms_norm(x, w).shape == (0, 64)
