@@ -126,8 +126,9 @@ def _activation(x, name: str = "x"):
     return dt, dev, shape[0], shape[1]
 
 
-def _call(name: str, dev: int, *args) -> None:
-    """The entry point with the current stream of device `dev`, on that device."""
+def _call(name: str, dev: int, *args, wrote=()) -> None:
+    """The entry point with the current stream of device `dev`, on that device.  `wrote`: the caller's tensors (or None)
+    that it writes, which autograd is told of."""
     fn = getattr(lib.load(), name)
     if torch.cuda.current_device() == dev:
         st = fn(*args, _stream(dev))
@@ -136,6 +137,9 @@ def _call(name: str, dev: int, *args) -> None:
             st = fn(*args, _stream(dev))
     if st != lib.RK_OK:
         lib.check(st, name)
+    for t in wrote:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
 
 
 def _q8_rows(like, rows: int, cols: int):
@@ -172,6 +176,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
     Returns y, or (y, h) when there is a residual or a `sum_out` (h in x's type; y comes from the unrounded sum).  `out`
     and `sum_out` may name tensors to write y and h to, x and residual themselves among them."""
     dt, dev, rows, cols, h, args = _norm_args(x, weight, residual, sum_out)
+    wrote = (out, sum_out)
     if out is None:
         out, ldy = x.new_empty((rows, cols)), cols
     else:
@@ -182,7 +187,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
         _apart(out, x, "out and x", itself=True)
         _apart(out, residual, "out and residual", itself=True)
         _apart(out, weight, "out and weight")
-    _call("rk_rms_norm", dev, *args, out.data_ptr(), ldy, rows, cols, eps, dt)
+    _call("rk_rms_norm", dev, *args, out.data_ptr(), ldy, rows, cols, eps, dt, wrote=wrote)
     return out if h is None else (out, h)
 
 
@@ -192,7 +197,8 @@ def rms_norm_q8(x, weight, residual=None, eps: float = 1e-6, sum_out=None):
     dt, dev, rows, cols, h, args = _norm_args(x, weight, residual, sum_out)
     q, ldq = _q8_rows(x, rows, cols)
     scale = x.new_empty((rows,), dtype=torch.float32)
-    _call("rk_rms_norm_q8", dev, *args, q.data_ptr(), ldq, scale.data_ptr(), rows, cols, eps, dt)
+    _call("rk_rms_norm_q8", dev, *args, q.data_ptr(), ldq, scale.data_ptr(), rows, cols, eps, dt,
+          wrote=(sum_out,))
     return (q, scale) if h is None else (q, scale, h)
 
 
@@ -256,9 +262,9 @@ def linear_q8(x, x_scale, w, w_scale, bias=None, residual=None, dtype=torch.floa
     pw, ldw = _q8_operand(w, "w", dev, n, k)
     sx = _vector(x_scale, "x_scale", torch.float32, dev, rows)
     sw = _vector(w_scale, "w_scale", torch.float32, dev, n)
-    out, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, x_scale=x_scale, w_scale=w_scale)
-    _call("rk_linear_q8", dev, px, ldx, sx, pw, ldw, sw, *tail, rows, n, k, dt)
-    return out
+    y, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, x_scale=x_scale, w_scale=w_scale)
+    _call("rk_linear_q8", dev, px, ldx, sx, pw, ldw, sw, *tail, rows, n, k, dt, wrote=(out,))
+    return y
 
 
 @functools.lru_cache(maxsize=4096)
@@ -323,12 +329,12 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
         if not (ldz == groups or n == 1):
             raise ValueError("zeros: a contiguous tensor is expected")
         zp = zeros.data_ptr()
-    out, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, scales=scales, zeros=zeros)
+    y, tail = _finish_args(rows, n, dtype, dev, bias, residual, out, x=x, w=w, scales=scales, zeros=zeros)
     size = _q4_workspace(rows, n, k, group, dt)
     ws = x.new_empty((size,), dtype=torch.uint8)  # torch's blocks start on 512-byte boundaries
     _call("rk_linear_q4", dev, x.data_ptr(), ldx, pw, ldw, scales.data_ptr(), zp, *tail, ws.data_ptr(), size, rows, n, k,
-          group, dt, st)
-    return out
+          group, dt, st, wrote=(out,))
+    return y
 
 
 def check(device: int | None = None) -> None:

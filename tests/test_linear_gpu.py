@@ -740,6 +740,30 @@ def test_outputs_that_overlap_weights_are_refused(lin):
     assert torch.equal(x, before)
 
 
+def test_autograd_is_told_of_tensors_written_in_place(lin):
+    """A tensor that autograd saved and a call then wrote to fails in the backward pass, as with torch's own functions."""
+    g = gen(24)
+    x, w = randn(g, 64, 64), randn(g, 64)
+    q, s = lin.quantize_q8(x)
+    p4, s4, _ = lin.quantize_q4(x, 32)
+    calls = [lambda t: lin.rms_norm(x, w, out=t), lambda t: lin.rms_norm(x, w, sum_out=t),
+             lambda t: lin.rms_norm(t, w, residual=x, sum_out=t), lambda t: lin.rms_norm_q8(x, w, sum_out=t),
+             lambda t: lin.linear_q8(q, s, q, s, out=t), lambda t: lin.linear_q4(x, p4, s4, 32, out=t),
+             lambda t: lin.linear_q4(x, p4, s4, 32, residual=t, out=t)]
+    for call in calls:
+        leaf = randn(g, 64, 64).requires_grad_()
+        saved = leaf.exp()  # its backward needs the result
+        with torch.no_grad():
+            call(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.sum().backward()
+    before = x._version
+    lin.rms_norm(x, w, residual=x)
+    assert x._version == before
+    with torch.inference_mode():
+        lin.rms_norm(x.clone(), w, out=torch.empty_like(x))
+
+
 def test_zero_rows(lin):
     x, w = torch.zeros(0, 64, device="cuda"), torch.ones(64, device="cuda")
     assert lin.rms_norm(x, w).shape == (0, 64)
