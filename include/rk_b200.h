@@ -153,7 +153,8 @@ RK_API rk_status rk_conv1d_static_check(void* stream);
  * may be x or residual themselves (same pitch).  weight has cols elements of
  * the same type.  _q8 writes 8-bit rows q [rows][cols] (pitch ldq bytes, a
  * multiple of 16 where rk_linear_q8 reads them; bytes between cols and ldq are
- * left as they are) and scale [rows]. */
+ * left as they are) and scale [rows].  Squares are summed in 32 bits: a row whose
+ * sum of squares passes 3.4e38 (values of 1e18 and more) gives zeros. */
 RK_API rk_status rk_rms_norm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight,
                              void* sum_out, long long lds, void* y, long long ldy, int rows, int cols, float eps,
                              int dtype, void* stream);
