@@ -3,6 +3,7 @@
 // bounded waits.
 #include "quant.cuh"
 
+#include <atomic>
 #include <cstdio>
 
 #include "status.h"
@@ -10,15 +11,15 @@
 namespace rk {
 
 int sm_count() {
-    static int cache[64] = {};
+    static std::atomic<int> cache[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (!cache[dev]) {
-        int n = 0;
+    int n = cache[dev].load(std::memory_order_relaxed);
+    if (!n) {
         cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        cache[dev] = n > 0 ? n : 148;
+        cache[dev].store(n = n > 0 ? n : 148, std::memory_order_relaxed);
     }
-    return cache[dev];
+    return n;
 }
 
 }  // namespace rk
