@@ -163,12 +163,6 @@ __global__ void __launch_bounds__(256) q4_parts_kernel(const Q4Args a, const Q4P
 
 __device__ uint32_t q4_err;  // set when a bounded wait of the kernel gives up
 
-__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
 // Four codes 0..15 in a word's bytes, z in each byte of `z`: q - z in e4m3, times 2^-9.  The bytes of u + 0x80 - z never
 // carry and keep the top bit where q >= z, which the sign is the inverse of.  (The negative side by complement and the
 // increments by mask, without vabsdiff4: two more instructions, 78 us for 75 at 4 x 16384 x 16384.)
@@ -239,7 +233,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1) linear_q4_kernel(const Q4Args a
             if (!mbar_wait_warp(&empty[s], parity, &q4_err, RK_DEV_TIMEOUT_EMPTY)) { lost = 1; break; }
             if (elect_one()) {
                 mbar_arrive_expect_tx(&full[s], p.x_bytes);
-                bulk_copy(ring + s * stage + Q4_A_BYTES, ws + (size_t)i * p.x_bytes, p.x_bytes, &full[s]);
+                bulk_load(ring + s * stage + Q4_A_BYTES, ws + (size_t)i * p.x_bytes, p.x_bytes, &full[s]);
             }
             if (++s == p.stages) { s = 0; parity ^= 1; }
         }
@@ -548,7 +542,7 @@ cudaError_t launch(const Q4Args& a, cudaStream_t st) {
     return launch_sub<T, 1>(a, st);
 }
 
-// largest finite value of a scale's type
+// A scale rounded to its type, at most the largest finite value there, as it is stored.
 __device__ __forceinline__ float store_scale(void* p, size_t i, float s, int dtype) {
     if (dtype == RK_DTYPE_F32) {
         static_cast<float*>(p)[i] = s;

@@ -51,9 +51,9 @@ void* q4_err_word();
 inline size_t dtype_bytes(int dtype) { return dtype == RK_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == RK_DTYPE_F32 || dtype == RK_DTYPE_F16 || dtype == RK_DTYPE_BF16; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-// a row pitch that holds `cols` elements (the pitch of a single row is never used)
 // Rows and columns up to 2^30: the kernels' 32-bit indices may step past an end by a tile or a block's width.
 inline bool size_ok(int n, int least) { return n >= least && n <= 1 << 30; }
+// a row pitch that holds `cols` elements (the pitch of a single row is never used)
 inline bool pitch_ok(long long ld, int rows, int cols) { return rows <= 1 || ld >= cols; }
 
 }  // namespace rk

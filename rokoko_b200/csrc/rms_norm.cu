@@ -183,13 +183,6 @@ __global__ void __launch_bounds__(G ? 256 : 1024) norm_rows_kernel(const NormArg
     }
 }
 
-// Bulk copy global -> shared of whole 16-byte granules, completion on `bar`.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
 // The 16-byte granules that hold a row; every granule holds at least one byte of it.
 __device__ __forceinline__ uint32_t granules(const void* row, uint32_t bytes, const char** first) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(row), lo = p & ~uintptr_t(15);
@@ -198,6 +191,33 @@ __device__ __forceinline__ uint32_t granules(const void* row, uint32_t bytes, co
 }
 
 constexpr int MAX_STAGES = 4;
+
+// The rows on their way to a block that walks over them: `stages` slots of shared memory, each for a row of x and one of
+// the residual behind it, whole granules.  One thread loads.
+struct RowRing {
+    uint8_t* slots;
+    uint64_t* bar;
+    int stages;
+    uint32_t slot_bytes, stage_bytes, row_bytes;
+    template <typename T>
+    __device__ __forceinline__ void load(const NormArgs& a, long long row, int s) const {
+        const char *px, *pr;
+        const uint32_t nx = granules(static_cast<const T*>(a.x) + row * a.ldx, row_bytes, &px);
+        uint32_t nr = 0;
+        if (a.res) nr = granules(static_cast<const T*>(a.res) + row * a.ldr, row_bytes, &pr);
+        mbar_arrive_expect_tx(&bar[s], nx + nr);
+        bulk_load(slots + (size_t)s * stage_bytes, px, nx, &bar[s]);
+        if (a.res) bulk_load(slots + (size_t)s * stage_bytes + slot_bytes, pr, nr, &bar[s]);
+    }
+    // A wait for slot s gave up at `row`: no copy may outlive the block.
+    __device__ __forceinline__ void drain(const NormArgs& a, long long row, long long step, int s, uint32_t parity) const {
+        for (int k = 0; k < stages; k++)
+            if (row + k * step < a.rows) {
+                const int q = s + k < stages ? s + k : s + k - stages;
+                mbar_wait(&bar[q], s + k < stages ? parity : parity ^ 1, &norm_err, RK_DEV_TIMEOUT_DRAIN);
+            }
+    }
+};
 
 // Many rows: resident blocks walk over the rows, the next rows of x and the
 // residual on their way into a ring of `stages` slots of shared memory (a bulk
@@ -216,26 +236,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     using P = Pack<T, VEC>;
     const int n = blockDim.x, tid = threadIdx.x;
     const long long step = gridDim.x;
-    const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
-    const uint32_t stage_bytes = slot_bytes * (a.res ? 2 : 1);
+    const RowRing ring{slots, bar, stages, slot_bytes, slot_bytes * (a.res ? 2 : 1), (uint32_t)a.cols * (uint32_t)sizeof(T)};
     if (tid == 0) {
         for (int s = 0; s < stages; s++) mbar_init(&bar[s], 1);
         fence_mbar_init();
     }
     __syncthreads();
-    auto load = [&](long long row, int s) {  // one thread
-        const char *px, *pr;
-        const uint32_t nx = granules(static_cast<const T*>(a.x) + row * a.ldx, row_bytes, &px);
-        uint32_t nr = 0;
-        if (a.res) nr = granules(static_cast<const T*>(a.res) + row * a.ldr, row_bytes, &pr);
-        mbar_arrive_expect_tx(&bar[s], nx + nr);
-        bulk_load(slots + (size_t)s * stage_bytes, px, nx, &bar[s]);
-        if (a.res) bulk_load(slots + (size_t)s * stage_bytes + slot_bytes, pr, nr, &bar[s]);
-    };
     long long row = blockIdx.x;
     if (tid == 0)
         for (int s = 0; s < stages; s++)
-            if (row + s * step < a.rows) load(row + s * step, s);
+            if (row + s * step < a.rows) ring.load<T>(a, row + s * step, s);
     P pw[NV];
     if (a.w) {
 #pragma unroll
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     bool ok = true;
     for (; row < a.rows; row += step) {
         ok = mbar_wait(&bar[s], parity, &norm_err, RK_DEV_TIMEOUT_FULL);
-        const uint8_t* slot = slots + (size_t)s * stage_bytes;
+        const uint8_t* slot = slots + (size_t)s * ring.stage_bytes;
         const T* x = reinterpret_cast<const T*>(slot + (VEC == 1 ? (uint32_t)((a.xoff + row * a.ldx * sizeof(T)) & 15) : 0));
         const T* r = reinterpret_cast<const T*>(slot + slot_bytes +
                                                 (VEC == 1 ? (uint32_t)((a.roff + row * a.ldr * sizeof(T)) & 15) : 0));
@@ -267,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         ok = p.reduce_block(red[flip], ok);
         flip ^= 1;
         if (!ok) break;  // the same for the whole block
-        if (tid == 0 && row + stages * step < a.rows) load(row + stages * step, s);
+        if (tid == 0 && row + stages * step < a.rows) ring.load<T>(a, row + stages * step, s);
         if (++s == stages) { s = 0; parity ^= 1; }
         const RowFactors f(a, p.ss, p.top);
         if (a.q && tid == 0) a.scale[row] = f.scale;
@@ -277,12 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
             if (c < a.cols) store_part<T, VEC>(a, row, c, hw[i], f);
         }
     }
-    if (!ok && tid == 0)  // a wait gave up: no copy may outlive the block
-        for (int k = 0; k < stages; k++)
-            if (row + k * step < a.rows) {
-                const int q = s + k < stages ? s + k : s + k - stages;
-                mbar_wait(&bar[q], s + k < stages ? parity : parity ^ 1, &norm_err, RK_DEV_TIMEOUT_DRAIN);
-            }
+    if (!ok && tid == 0) ring.drain(a, row, step, s, parity);
 }
 
 // norm_stream_kernel for rows off the 16-byte grid.  Elements are worked on where
@@ -305,26 +310,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     const int tid = threadIdx.x, lane = tid & 31;
     const int first = tid / 32 * (32 * NV) + lane;  // a warp's vectors lie together
     const long long step = gridDim.x;
-    const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T), stage_bytes = slot_bytes * (a.res ? 2 : 1);
+    const RowRing ring{slots, bar, stages, slot_bytes, slot_bytes * (a.res ? 2 : 1), (uint32_t)a.cols * (uint32_t)sizeof(T)};
     const int skip = (int)((a.xoff + (long long)blockIdx.x * a.ldx * (long long)sizeof(T)) & 15) / (int)sizeof(T);
     if (tid == 0) {
         for (int s = 0; s < stages; s++) mbar_init(&bar[s], 1);
         fence_mbar_init();
     }
     __syncthreads();
-    auto load = [&](long long row, int s) {  // one thread
-        const char *px, *pr;
-        const uint32_t nx = granules(static_cast<const T*>(a.x) + row * a.ldx, row_bytes, &px);
-        uint32_t nr = 0;
-        if (a.res) nr = granules(static_cast<const T*>(a.res) + row * a.ldr, row_bytes, &pr);
-        mbar_arrive_expect_tx(&bar[s], nx + nr);
-        bulk_load(slots + (size_t)s * stage_bytes, px, nx, &bar[s]);
-        if (a.res) bulk_load(slots + (size_t)s * stage_bytes + slot_bytes, pr, nr, &bar[s]);
-    };
     long long row = blockIdx.x;
     if (tid == 0)
         for (int s = 0; s < stages; s++)
-            if (row + s * step < a.rows) load(row + s * step, s);
+            if (row + s * step < a.rows) ring.load<T>(a, row + s * step, s);
     P pw[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -338,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     bool ok = true;
     for (; row < a.rows; row += step) {
         ok = mbar_wait(&bar[s], parity, &norm_err, RK_DEV_TIMEOUT_FULL);
-        const uint8_t* slot = slots + (size_t)s * stage_bytes;
+        const uint8_t* slot = slots + (size_t)s * ring.stage_bytes;
         float hw[NV][VEC];
         RowPart<T, VEC> p;
 #pragma unroll
@@ -369,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         ok = p.reduce_block(red[flip], ok);
         flip ^= 1;
         if (!ok) break;  // the same for the whole block
-        if (tid == 0 && row + stages * step < a.rows) load(row + stages * step, s);
+        if (tid == 0 && row + stages * step < a.rows) ring.load<T>(a, row + stages * step, s);
         if (++s == stages) { s = 0; parity ^= 1; }
         const RowFactors f(a, p.ss, p.top);
         if (a.q && tid == 0) a.scale[row] = f.scale;
@@ -426,12 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
             }
         }
     }
-    if (!ok && tid == 0)  // a wait gave up: no copy may outlive the block
-        for (int k = 0; k < stages; k++)
-            if (row + k * step < a.rows) {
-                const int q = s + k < stages ? s + k : s + k - stages;
-                mbar_wait(&bar[q], s + k < stages ? parity : parity ^ 1, &norm_err, RK_DEV_TIMEOUT_DRAIN);
-            }
+    if (!ok && tid == 0) ring.drain(a, row, step, s, parity);
 }
 
 // Rows that do not fit one block's registers: read twice, the second time from L2.
