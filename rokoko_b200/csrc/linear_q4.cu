@@ -26,7 +26,10 @@
 // whose parts are N columns of their own: an MMA takes 66 clocks whatever N <=
 // 112 is, so its rows are what must not lie idle.  Some warps turn codes into
 // operands, one thread issues the MMAs, eight warps add up the accumulators.  The
-// weights' bytes are read once.
+// weights' bytes are read once.  Bound by the latency of a step in the warps of
+// codes, with small groups by that of reading accumulators back: 1 x 8192 x 8192
+// bf16 21.8 us, 4 x 16384 x 16384 half with zero points 75 us (1.9 TB/s), 24 x
+// 5003 x 4001 float in groups of 32 72 us.
 //
 // A row with an infinity, a NaN, or magnitudes too far apart does not fit the
 // parts; its sums are done one by one in 32 bits instead.

@@ -300,7 +300,8 @@ def linear_q4(x, w, scales, group: int, zeros=None, bias=None, residual=None, ou
     group)], zeros of the same shape or None); the result in x's type.
 
     bias is float32 [n], residual [rows, n] in x's type; `out` may name the tensor to write, residual itself among
-    them.  For few rows: the cost is the weights' bytes."""
+    them.  For few rows: the cost is the weights' bytes.  A row of x whose magnitudes lie too far apart (2^30, half 2^27),
+    with an infinity or a NaN takes far longer (include/rk_b200.h)."""
     dt, dev, rows, k = _activation(x)
     dtype = x.dtype
     ldx = _rows(x, "x", dtype, dev, rows, k)
